@@ -25,6 +25,7 @@
 
 #include "custom_call.h"
 #include "kernels/attention.h"
+#include "operators.h"
 #include "planner.h"
 #include "runtime.h"
 
@@ -37,6 +38,7 @@ constexpr const char* kSdpaTarget = "pjrtx.mlx_metal.scaled_dot_product_attentio
 bool is_attention_float(DType t) { return t == DType::kF32 || t == DType::kF16 || t == DType::kBF16; }
 
 void lower_custom_call(Program* prog, Op* op) {
+  if (lower_operator_call(*prog, op)) return;
   if (op->target != kSdpaTarget) {
     // Registered identity / unary / binary targets (custom_call.cc).
     lower_registered_custom_call(*prog, op);

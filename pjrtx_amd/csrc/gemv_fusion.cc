@@ -171,6 +171,8 @@ bool written_between(const Program& prog, const std::vector<Step>& steps, size_t
     for (auto& [pos, ww] : s.window_out)
       if (ww.operand == v) return true;
     if (s.kind == StepKind::kLibrary && s.in_place && prog.ops[s.lib_op].operands[0] == v) return true;
+    for (size_t k = 0; s.in_place_operands >> k; ++k)
+      if ((s.in_place_operands >> k & 1) && prog.ops[s.lib_op].operands[k] == v) return true;
   }
   return false;
 }

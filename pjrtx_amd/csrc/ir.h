@@ -55,6 +55,8 @@ enum class OpKind {
   // fused attention op that the program rewrite produces from a
   // scaled-dot-product-attention custom call or the unfused pattern.
   kCustomCall, kAttention,
+  // operator custom calls (operators.cc lists operands, results, attributes)
+  kPagedAttention, kPagedAppend, kAddRmsNorm, kAddRmsNormGrad, kTokenLogprobs, kTokenLogprobsGrad,
   kReturn,
 };
 
@@ -83,6 +85,14 @@ struct AttentionAttrs {
   int64_t offset = 0;
   bool has_offset_operand = false;
   bool round_scores = false;
+};
+
+// The operator custom calls' configuration.
+struct OperatorAttrs {
+  double scale = 1.0;   // paged attention
+  int64_t window = 0;   // paged attention: last keys attended, 0 for all
+  double eps = 0.0;     // norm and its gradient
+  int64_t top_k = 0;    // token log probabilities
 };
 
 struct Op {
@@ -142,9 +152,12 @@ struct Op {
   // reduce / scatter body
   std::vector<Region> regions;
 
-  // custom_call target name; kAttention attributes
+  // custom_call target name and the entries of its backend_config
+  // dictionary; kAttention attributes; the operators' configuration
   std::string target;
+  std::map<std::string, std::string> config;
   AttentionAttrs attn;
+  OperatorAttrs oper;
 };
 
 struct Region {

@@ -1,0 +1,59 @@
+// Vector loads and stores of tensor elements as floats. Rows of any length
+// start at any element, so a vector is aligned to its element only (global
+// memory takes 16 bytes at any address).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace pjrtx {
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+// kVec elements of T are 16 bytes.
+template <typename T>
+constexpr int kVecElems = 16 / (int)sizeof(T);
+
+template <typename T>
+struct Vec {
+  typedef T type __attribute__((ext_vector_type(kVecElems<T>)));
+  typedef type unaligned __attribute__((aligned(sizeof(T))));
+};
+
+// Elements [0, n) of the vector at p, the others `fill`. n >= kVecElems is the
+// common case: one load.
+template <typename T>
+__device__ __forceinline__ typename Vec<T>::type load_vec(const T* p, int64_t n, T fill) {
+  if (n >= kVecElems<T>) return *reinterpret_cast<const typename Vec<T>::unaligned*>(p);
+  typename Vec<T>::type v;
+#pragma unroll
+  for (int e = 0; e < kVecElems<T>; ++e) v[e] = e < n ? p[e] : fill;
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_vec(T* p, int64_t n, const typename Vec<T>::type& v) {
+  if (n >= kVecElems<T>) {
+    *reinterpret_cast<typename Vec<T>::unaligned*>(p) = v;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < kVecElems<T>; ++e)
+    if (e < n) p[e] = v[e];
+}
+
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+  for (int k = 32; k >= 1; k >>= 1) x += __shfl_xor(x, k);
+  return x;
+}
+// NaN where any lane's is.
+__device__ __forceinline__ float wave_max_nan(float x) {
+#pragma unroll
+  for (int k = 32; k >= 1; k >>= 1) x = __builtin_elementwise_maximum(x, __shfl_xor(x, k));
+  return x;
+}
+
+}  // namespace pjrtx

@@ -2,6 +2,7 @@
 // through a precompiled kernel instead of a generated fusion.
 #include "kernels/library.h"
 #include "kernels/reduce_window.h"
+#include "operators.h"
 
 #include <cstring>
 #include <map>
@@ -369,6 +370,10 @@ void run_library_step(Device* dev, const Program& prog, const Step& step, std::v
       run_reduce_window(dev, prog, op, vals);
       return;
     default:
+      if (operator_lib_kind(op.kind) != LibKind::kCopy) {
+        run_operator(dev, prog, step, vals);
+        return;
+      }
       fail(Code::kUnimplemented, std::string("library op not available: ") + lib_kind_name(step.lib));
   }
 }

@@ -181,7 +181,16 @@ bool lookup_op(const std::string& mnemonic, OpKind* out) {
 }  // namespace
 
 const char* op_kind_name(OpKind k) {
-  if (k == OpKind::kParameter) return "parameter";
+  switch (k) {
+    case OpKind::kParameter: return "parameter";
+    case OpKind::kPagedAttention: return "pjrtx.paged_attention";
+    case OpKind::kPagedAppend: return "pjrtx.paged_append";
+    case OpKind::kAddRmsNorm: return "pjrtx.add_rms_norm";
+    case OpKind::kAddRmsNormGrad: return "pjrtx.add_rms_norm_grad";
+    case OpKind::kTokenLogprobs: return "pjrtx.token_logprobs";
+    case OpKind::kTokenLogprobsGrad: return "pjrtx.token_logprobs_grad";
+    default: break;
+  }
   for (const OpInfo& info : kOpTable) {
     if (info.kind == k) return info.mnemonic;
   }
@@ -996,6 +1005,8 @@ void Parser::parse_generic_attrs(const std::string& dict, Op* op) {
     } else if (key == "call_target_name") {
       const size_t q0 = val.find('"'), q1 = val.rfind('"');
       if (q0 != std::string::npos && q1 > q0) op->target = val.substr(q0 + 1, q1 - q0 - 1);
+    } else if (key == "backend_config" && op->kind == OpKind::kCustomCall && val.size() >= 2 && val[0] == '{') {
+      op->config = split_attr_dict(val.substr(1, val.rfind('}') - 1));
     } else if (key == "dot_dimension_numbers") {
       size_t lt = val.find('<');
       size_t gt = val.rfind('>');

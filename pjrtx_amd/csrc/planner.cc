@@ -1,5 +1,6 @@
 // Fusion planner implementation. See planner.h for the contract.
 #include "kernels/dot.h"
+#include "operators.h"
 #include "planner.h"
 #include "sort_op.h"
 
@@ -39,6 +40,12 @@ const char* lib_kind_name(LibKind k) {
     case LibKind::kAttention: return "attention";
     case LibKind::kDotGroup: return "dot_group";
     case LibKind::kWhile: return "while";
+    case LibKind::kPagedAttention: return "paged_attention";
+    case LibKind::kPagedAppend: return "paged_append";
+    case LibKind::kAddRmsNorm: return "add_rms_norm";
+    case LibKind::kAddRmsNormGrad: return "add_rms_norm_grad";
+    case LibKind::kTokenLogprobs: return "token_logprobs";
+    case LibKind::kTokenLogprobsGrad: return "token_logprobs_grad";
     case LibKind::kSort: return "sort";
     case LibKind::kReduceWindow: return "reduce_window";
   }
@@ -186,7 +193,8 @@ bool is_library(const Op& op) {
   return k == OpKind::kDotGeneral || k == OpKind::kGather || k == OpKind::kScatter ||
          k == OpKind::kDynamicSlice || k == OpKind::kDynamicUpdateSlice ||
          (k == OpKind::kConcatenate && !fusible_concat(op)) || k == OpKind::kPad || k == OpKind::kAttention ||
-         k == OpKind::kWhile || k == OpKind::kSort || k == OpKind::kTopK || k == OpKind::kReduceWindow;
+         k == OpKind::kWhile || k == OpKind::kSort || k == OpKind::kTopK || k == OpKind::kReduceWindow ||
+         operator_lib_kind(k) != LibKind::kCopy;
 }
 
 LibKind lib_kind_of(OpKind k) {
@@ -203,7 +211,7 @@ LibKind lib_kind_of(OpKind k) {
     case OpKind::kSort:
     case OpKind::kTopK: return LibKind::kSort;
     case OpKind::kReduceWindow: return LibKind::kReduceWindow;
-    default: return LibKind::kCopy;
+    default: return operator_lib_kind(k);
   }
 }
 
@@ -1068,14 +1076,21 @@ void Planner::liveness() {
   }
   for (size_t i = 0; i < plan_.steps.size(); ++i) {
     Step& s = plan_.steps[i];
-    if (s.kind != StepKind::kLibrary || s.lib != LibKind::kDynamicUpdateSlice) continue;
-    const int v0 = prog_.ops[s.lib_op].operands[0];
-    const bool intermediate = !persistent.count(v0) && !outputs_.count(v0) && !aliased.count(v0) &&
-                              producer_kind.count(v0) && producer_kind[v0] != StepKind::kAlias;
-    const bool donated = donated_param.count(v0) && !outputs_.count(v0) && !aliased.count(v0);
-    if ((intermediate || donated) && last_use[v0] == static_cast<int>(i)) {
-      s.in_place = true;
-      if (donated) plan_.written_params.push_back(donated_param[v0]);
+    const bool append = s.kind == StepKind::kLibrary && s.lib == LibKind::kPagedAppend;
+    if (!append && (s.kind != StepKind::kLibrary || s.lib != LibKind::kDynamicUpdateSlice)) continue;
+    const std::vector<int>& operands = prog_.ops[s.lib_op].operands;
+    for (size_t k = 0; k < (append ? 2u : 1u); ++k) {
+      const int v0 = operands[k];
+      // paged_append: the keys' pages and the values' may be one value.
+      if (std::count(operands.begin(), operands.end(), v0) > 1 && append) continue;
+      const bool intermediate = !persistent.count(v0) && !outputs_.count(v0) && !aliased.count(v0) &&
+                                producer_kind.count(v0) && producer_kind[v0] != StepKind::kAlias;
+      const bool donated = donated_param.count(v0) && !outputs_.count(v0) && !aliased.count(v0);
+      if ((intermediate || donated) && last_use[v0] == static_cast<int>(i)) {
+        if (append) s.in_place_operands |= 1u << k;
+        else s.in_place = true;
+        if (donated) plan_.written_params.push_back(donated_param[v0]);
+      }
     }
   }
 }
@@ -1403,6 +1418,12 @@ std::string Plan::describe(const Program& prog) const {
       } else if (s.lib == LibKind::kDynamicUpdateSlice && s.in_place) {
         alg = 2 * prog.type(d.operands[1]).bytes();
         for (size_t k = 2; k < d.operands.size(); ++k) alg += prog.type(d.operands[k]).bytes();
+      } else if (s.lib == LibKind::kPagedAppend) {
+        // The new rows read and written; pages that are not written in place
+        // are copied.
+        alg = 2 * (prog.type(d.operands[2]).bytes() + prog.type(d.operands[3]).bytes()) + prog.type(d.operands[4]).bytes();
+        for (int k = 0; k < 2; ++k)
+          if (!(s.in_place_operands & (1u << k))) alg += 2 * prog.type(d.operands[k]).bytes();
       }
     }
     if (s.kind == StepKind::kGemv) {
@@ -1483,6 +1504,7 @@ std::string Plan::describe(const Program& prog) const {
         o << ",\"scratch_bytes\":" << sort_op_scratch(prog, prog.ops[s.lib_op], int64_t(1) << 60)
           << ",\"least_scratch_bytes\":" << sort_op_scratch(prog, prog.ops[s.lib_op], 0);
       if (s.lib == LibKind::kWhile) o << ",\"while_trips\":" << s.while_trips;
+      if (s.lib == LibKind::kPagedAppend) o << ",\"in_place_operands\":" << s.in_place_operands;
       if (s.lib == LibKind::kAttention) {  // q.k and p.v over every (query, key) pair
         const Op& d = prog.ops[s.lib_op];
         const TensorType& q = prog.type(d.operands[0]);

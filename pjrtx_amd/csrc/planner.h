@@ -57,7 +57,7 @@ enum class StepKind { kLoop, kReduce, kAlias, kLibrary, kRowFused, kGemv };
 
 enum class LibKind {
   kCopy, kDot, kGather, kScatter, kDynamicSlice, kDynamicUpdateSlice, kConcatenate, kPad, kAttention, kDotGroup, kWhile, kSort,
-  kReduceWindow
+  kReduceWindow, kPagedAttention, kPagedAppend, kAddRmsNorm, kAddRmsNormGrad, kTokenLogprobs, kTokenLogprobsGrad
 };
 const char* lib_kind_name(LibKind k);
 
@@ -132,6 +132,9 @@ struct Step {
   // dynamic_update_slice whose operand dies here: the update is written into
   // the operand's buffer, which becomes the result (no copy).
   bool in_place = false;
+  // paged_append: bit k set where result k is written into operand k's buffer
+  // (the operand dies here).
+  uint32_t in_place_operands = 0;
   // kAttention on the split decode path whose only reader is a kGemv that
   // merges the splits: the output buffer holds the split partials
   // (attention_partials_bytes), not the output rows.

@@ -2,6 +2,7 @@
 #include "runtime.h"
 #include "kernels/library.h"
 #include "kernels/noalloc.h"
+#include "operators.h"
 
 #include <hip/hiprtc.h>
 #include <sys/stat.h>
@@ -938,7 +939,8 @@ class StepTemporaries {
 };
 }  // namespace
 
-void Executable::run_step(Loaded* L, size_t si, std::vector<MemRef>& vals, int phase) {
+void Executable::run_step(Loaded* L, size_t si, std::vector<MemRef>& vals, int phase,
+                          const std::vector<MemRef>* placed) {
   const Step& s = plan_.steps[si];
   Device* dev = L->dev;
   switch (s.kind) {
@@ -955,7 +957,13 @@ void Executable::run_step(Loaded* L, size_t si, std::vector<MemRef>& vals, int p
       } else if (s.attn_partials) {
         vals[s.outputs[0]] = dev->allocate(attention_partials_bytes(prog_, prog_.ops[s.lib_op]));
       } else {
-        for (int v : s.outputs) vals[v] = dev->allocate(prog_.type(v).bytes());
+        const std::vector<int>& operands = prog_.ops[s.lib_op].operands;
+        for (size_t k = 0; k < s.outputs.size(); ++k) {
+          const int v = s.outputs[k];
+          if (k < 32 && (s.in_place_operands >> k & 1)) vals[v] = vals[operands[k]];
+          else if (placed && (*placed)[v]) vals[v] = (*placed)[v];
+          else vals[v] = dev->allocate(prog_.type(v).bytes());
+        }
       }
       {
         StepTemporaries temporaries(thread_arena());
@@ -1158,7 +1166,56 @@ size_t Executable::execute_noalloc(Device* dev, const void* const* args, size_t 
     m->borrowed = true;
     vals[prog_.params[i]] = m;
   }
+  // Results that go straight to the caller's memory.
+  auto overlaps = [](const void* a, size_t na, const void* b, size_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return na && nb && x < y + nb && y < x + na;
+  };
+  auto alone = [&](size_t i, int param) {  // output i against all arguments (but `param`) and other outputs
+    const size_t n = prog_.type(prog_.results[i]).bytes();
+    for (size_t k = 0; k < num_args; ++k)
+      if (static_cast<int>(k) != param && overlaps(outs[i], n, args[k], prog_.type(prog_.params[k]).bytes())) return false;
+    for (size_t k = 0; k < num_outs; ++k)
+      if (k != i && overlaps(outs[i], n, outs[k], prog_.type(prog_.results[k]).bytes())) return false;
+    return n > 0;
+  };
+  // Whether `result` is parameter k's buffer after the plan's in-place writes.
+  auto keeps_buffer = [&](int k, int result) {
+    std::set<int> held = {prog_.params[k]};
+    for (const Step& st : plan_.steps) {
+      if (st.kind == StepKind::kAlias && held.count(st.inputs[0])) held.insert(st.outputs[0]);
+      for (const auto& [pos, ww] : st.window_out)
+        if (held.count(ww.operand)) held.insert(st.outputs[pos]);
+      if (st.kind != StepKind::kLibrary) continue;
+      const Op& op = prog_.ops[st.lib_op];
+      if (st.in_place && held.count(op.operands[0])) held.insert(st.outputs[0]);
+      for (size_t i = 0; st.in_place_operands >> i; ++i)
+        if ((st.in_place_operands >> i & 1) && held.count(op.operands[i])) held.insert(st.outputs[i]);
+    }
+    return held.count(result) > 0;
+  };
+  std::vector<MemRef> placed(prog_.values.size());
+  for (const Step& st : plan_.steps) {
+    if (st.kind != StepKind::kLibrary || operator_lib_kind(prog_.ops[st.lib_op].kind) == LibKind::kCopy) continue;
+    for (int v : st.outputs) {
+      const auto first = std::find(prog_.results.begin(), prog_.results.end(), v);
+      if (first == prog_.results.end() || std::count(first, prog_.results.end(), v) > 1) continue;
+      const size_t i = first - prog_.results.begin();
+      if (!alone(i, -1)) continue;
+      auto m = std::make_shared<DeviceMemory>();
+      m->dev = dev;
+      m->ptr = outs[i];
+      m->bytes = m->capacity = prog_.type(v).bytes();
+      m->borrowed = true;
+      placed[v] = m;
+    }
+  }
   for (int k : plan_.written_params) {
+    const int64_t to = prog_.param_alias.at(k);
+    if (to >= 0 && to < static_cast<int64_t>(num_outs) && outs[to] == args[k] &&
+        prog_.type(prog_.results[to]) == prog_.type(prog_.params[k]) && alone(to, k) &&
+        keeps_buffer(k, prog_.results[to]))
+      continue;  // given back in the same memory: written where it is
     // The plan writes this parameter in place: work on a copy, the caller's
     // input stays as it was.
     const MemRef& src = vals[prog_.params[k]];
@@ -1170,7 +1227,7 @@ size_t Executable::execute_noalloc(Device* dev, const void* const* args, size_t 
   }
   for (auto& [v, m] : L->constants) vals[v] = m;
   for (size_t si = 0; si < plan_.steps.size(); ++si) {
-    run_step(L, si, vals);
+    run_step(L, si, vals, -1, &placed);
     for (int v : plan_.steps[si].release_after) vals[v].reset();
   }
   for (size_t i = 0; i < num_outs; ++i) {

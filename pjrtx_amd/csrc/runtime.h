@@ -312,7 +312,11 @@ class Executable {
   // and outs[i] are device addresses of the parameter / result sizes; every
   // intermediate, copy of a parameter the plan writes, and kernel scratch
   // block comes from the device's fixed no-allocation block (kernels/
-  // noalloc.h), whose contents the previous call left behind. Work is queued
+  // noalloc.h), whose contents the previous call left behind. A result that
+  // an operator's step produces is written straight to its output, and an
+  // output at the address of the donated argument that the plan writes in
+  // place for it (the argument's `tf.aliasing_output`) is written there, where
+  // no other argument or output of the call overlaps either. Work is queued
   // on the device stream (no graph capture, no completion event). The
   // executable must already be loaded on `dev`. Returns the arena bytes used.
   size_t execute_noalloc(Device* dev, const void* const* args, size_t num_args, void* const* outs,
@@ -402,7 +406,10 @@ class Executable {
                                       std::shared_ptr<Event>* done);
   // phase: -1 runs the whole step; 0 only the main kernel of a split
   // reduction, 1 only its combine kernel (outputs must already exist).
-  void run_step(Loaded* L, size_t si, std::vector<MemRef>& vals, int phase = -1);
+  // placed[v], when given and set, is the memory of value v, which a step then
+  // writes instead of a block of its own.
+  void run_step(Loaded* L, size_t si, std::vector<MemRef>& vals, int phase = -1,
+                const std::vector<MemRef>* placed = nullptr);
 };
 
 // Library steps (dot_general, gather, scatter, dynamic slices, ...).

@@ -365,6 +365,84 @@ class Builder:
         return self._emit(f'stablehlo.custom_call @{target}({names}) {{api_version = 2 : i32, backend_config = ""}} : '
                           f"({types}) -> {out}", shape, dtype)
 
+    def operator_call(self, target: str, operands: list[T], results: list[tuple], config: dict | None = None) -> list[T]:
+        """stablehlo.custom_call with attributes, as jax.ffi.ffi_call prints it.
+        `results`: (shape, dtype) of each."""
+        def attr(v):
+            return f"{v} : i64" if isinstance(v, int) else f"{v:.17e} : f64"
+        cfg = ", ".join(f"{k} = {attr(v)}" for k, v in (config or {}).items())
+        names = ", ".join(o.name for o in operands)
+        types = ", ".join(o.type for o in operands)
+        outs = ", ".join(tensor_type(s, d) for s, d in results)
+        outs = outs if len(results) == 1 else f"({outs})"
+        name = self._fresh()
+        res = name if len(results) == 1 else f"{name}:{len(results)}"
+        self.lines.append(f"    {res} = stablehlo.custom_call @{target}({names}) {{api_version = 4 : i32, "
+                          f"backend_config = {{{cfg}}}}} : ({types}) -> {outs}")
+        if len(results) == 1:
+            return [T(name, tuple(results[0][0]), results[0][1])]
+        return [T(f"{name}#{i}", tuple(s), d) for i, (s, d) in enumerate(results)]
+
+    def paged_attention(self, q: T, k_pages: T, v_pages: T, page_table: T, lengths: T, scale: float | None = None,
+                        window: int = 0) -> T:
+        """Attention of one new token a sequence, q [B, Hq, D], over a paged
+        cache [P, Hkv, S, D]. Sequence b's key j lies in page
+        page_table[b, j // S] at j % S; keys lengths[b] - window (0 when window
+        is 0) to lengths[b] - 1 are attended, but for those whose page is
+        outside [0, P). A sequence with none answers zeros. `scale` defaults to
+        1 / sqrt(D)."""
+        config = {} if scale is None else {"scale": float(scale)}
+        if window:
+            config["window"] = int(window)
+        return self.operator_call("pjrtx.paged_attention", [q, k_pages, v_pages, page_table, lengths],
+                                  [(q.shape, q.dtype)], config)[0]
+
+    def paged_append(self, k_pages: T, v_pages: T, k_new: T, v_new: T, slots: T) -> tuple[T, T]:
+        """The pages with row n of k_new / v_new [N, Hkv, D] written at slot
+        slots[n] = page * S + position. A slot outside the pages leaves its row
+        out; of rows that name one slot the last stays. Donated pages are
+        written where they are."""
+        k, v = self.operator_call("pjrtx.paged_append", [k_pages, v_pages, k_new, v_new, slots],
+                                  [(k_pages.shape, k_pages.dtype), (v_pages.shape, v_pages.dtype)])
+        return k, v
+
+    def add_rms_norm(self, x: T, residual: T | None, gain: T, eps: float = 1e-5, quantize: bool = False) -> tuple:
+        """t = x + residual, y = t * gain / sqrt(mean(t^2) + eps) over the last
+        dim: (y, t). `quantize`: (y in s8, its f32 scales max|y| / 127 a row,
+        t). Without a residual t is x, and is not returned."""
+        results = [(x.shape, "s8"), (x.shape[:-1], "f32")] if quantize else [(x.shape, x.dtype)]
+        operands = [x, gain]
+        if residual is not None:
+            operands = [x, residual, gain]
+            results.append((x.shape, x.dtype))
+        return tuple(self.operator_call("pjrtx.add_rms_norm", operands, results, {"eps": float(eps)}))
+
+    def add_rms_norm_grad(self, dy: T, dsum: T | None, total: T, gain: T, eps: float = 1e-5) -> tuple[T, T]:
+        """The gradients (dx, dgain) of add_rms_norm from those of its results,
+        the norm's `dy` and the sum's `dsum` (or None), and from the sum
+        `total` it gave. dx is the gradient of x and of the residual."""
+        operands = [dy, total, gain] if dsum is None else [dy, dsum, total, gain]
+        dx, dgain = self.operator_call("pjrtx.add_rms_norm_grad", operands,
+                                       [(dy.shape, dy.dtype), (gain.shape, gain.dtype)], {"eps": float(eps)})
+        return dx, dgain
+
+    def token_logprobs(self, logits: T, tokens: T, top_k: int = 0) -> tuple:
+        """Of each row of logits [N, V], in f32: the log probability of its
+        token (0 for a token outside [0, V)), the distribution's entropy, the
+        log of the sum of exponentials; with top_k the likeliest tokens' log
+        probabilities and their s32 ids (ties to the lowest) [N, top_k]."""
+        n = logits.shape[0]
+        results = [((n,), "f32")] * 3
+        if top_k:
+            results += [((n, top_k), "f32"), ((n, top_k), "s32")]
+        return tuple(self.operator_call("pjrtx.token_logprobs", [logits, tokens], results))
+
+    def token_logprobs_grad(self, logits: T, tokens: T, lse: T, entropy: T, d_logprobs: T, d_entropy: T) -> T:
+        """The logits' gradient from those of token_logprobs' log probabilities
+        and entropies (f32 [N]), and the lse and entropy it gave."""
+        return self.operator_call("pjrtx.token_logprobs_grad", [logits, tokens, lse, entropy, d_logprobs, d_entropy],
+                                  [(logits.shape, logits.dtype)])[0]
+
     def pad(self, x: T, value: T, low, high, interior) -> T:
         shape = tuple(lo + hi + d + max(d - 1, 0) * it for d, lo, hi, it in zip(x.shape, low, high, interior))
         f = lambda v: ", ".join(str(a) for a in v)  # noqa: E731
