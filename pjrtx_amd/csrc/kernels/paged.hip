@@ -14,6 +14,7 @@
 // unnormalised output) to scratch; paged_combine folds them in split order.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "kernels/operators.h"
 #include "kernels/vec.h"
@@ -157,38 +158,43 @@ __device__ __forceinline__ float* slot_state(const Shape& s, float* scratch, int
   return scratch + slot * s.heads * (s.p.D + 2);
 }
 
-// The workgroup's waves meet over one head: state of wave w in ml[w], its
-// outputs in o[w]. Writes the row's result, or the split's partial one.
+// The workgroup's waves meet: the state of head h in wave w is ml[w][h], a sum
+// of -1 where the wave attended no key, and its outputs are o[(w heads + h) D].
+// Writes the rows' results, or the split's partial ones, of the unit's heads
+// first .. first + heads - 1.
 template <typename T>
-__device__ __forceinline__ void finish_head(const Shape& s, const Unit& u, int head, const float (*ml)[2],
-                                            const float* o, int o_stride, T* out, float* scratch) {
-  float m = -INFINITY;
-  bool any = false;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (ml[w][1] < 0.f) continue;
-    any = true;
-    m = fmaxf(m, ml[w][0]);
-  }
-  const float ref = m == -INFINITY ? 0.f : m;
-  float f[kWaves], l = 0.f;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    f[w] = ml[w][1] < 0.f ? 0.f : exp2f(ml[w][0] - ref);
-    l += ml[w][1] < 0.f ? 0.f : ml[w][1] * f[w];
-  }
+__device__ __forceinline__ void finish_heads(const Shape& s, const Unit& u, int first, int heads,
+                                             const float (*ml)[kHeads][2], const float* o, T* out, float* scratch) {
+  const int D = s.p.D;
   float* state = u.n > 1 ? slot_state(s, scratch, u.slot) : nullptr;
-  if (state && threadIdx.x == 0) {
-    state[2 * head] = m;
-    state[2 * head + 1] = any ? l : -1.f;
-  }
-  for (int d = threadIdx.x; d < s.p.D; d += kWaves * 64) {
-    float v = 0.f;
+  for (int i = threadIdx.x; i < heads * D; i += kWaves * 64) {
+    const int h = i / D, d = i - h * D, hu = first + h;
+    float m = -INFINITY;
+    bool any = false;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w)
-      if (ml[w][1] >= 0.f || ml[w][1] != ml[w][1]) v += f[w] * o[w * o_stride + d];
-    if (state) state[2 * s.heads + (int64_t)head * s.p.D + d] = v;
-    else out[(u.b * s.p.Hq + u.head0 + head) * s.p.D + d] = (T)(any ? v / l : 0.f);
+    for (int w = 0; w < kWaves; ++w) {
+      const bool none = ml[w][h][1] < 0.f;
+      any = any || !none;
+      m = none ? m : fmaxf(m, ml[w][h][0]);
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f, v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      if (ml[w][h][1] < 0.f) continue;  // its outputs were not written
+      const float f = exp2f(ml[w][h][0] - ref);
+      l += ml[w][h][1] * f;
+      v += o[(w * heads + h) * D + d] * f;
+    }
+    if (!state) {
+      out[(u.b * s.p.Hq + u.head0 + hu) * D + d] = (T)(any ? v / l : 0.f);
+      continue;
+    }
+    if (d == 0) {
+      state[2 * hu] = m;
+      state[2 * hu + 1] = any ? l : -1.f;
+    }
+    state[2 * s.heads + (int64_t)hu * D + d] = v;
   }
 }
 
@@ -201,8 +207,8 @@ __global__ void __launch_bounds__(kWaves * 64)
               const int32_t* __restrict__ table, const int32_t* __restrict__ lengths, T* __restrict__ out,
               float* __restrict__ scratch) {
   constexpr int J = kMaxHeadDim / 64;
-  __shared__ float ml[kWaves][2];
-  __shared__ float ow[kWaves][kMaxHeadDim];
+  __shared__ float ml[kWaves][kHeads][2];
+  __shared__ float ow[kWaves * kMaxHeadDim];  // [waves][D]
   Unit u;
   if (!find_unit(s, lengths, &u)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -242,16 +248,321 @@ __global__ void __launch_bounds__(kWaves * 64)
       }
     }
     if (lane == 0) {
-      ml[wave][0] = m;
-      ml[wave][1] = l;
+      ml[wave][0][0] = m;
+      ml[wave][0][1] = l;
     }
 #pragma unroll
     for (int j = 0; j < J; ++j)
-      if (lane + 64 * j < D) ow[wave][lane + 64 * j] = o[j];
+      if (lane + 64 * j < D) ow[wave * D + lane + 64 * j] = o[j];
     __syncthreads();
-    finish_head<T>(s, u, h, ml, ow[0], kMaxHeadDim, out, scratch);
+    finish_heads<T>(s, u, h, 1, ml, ow, out, scratch);
     __syncthreads();
   }
+}
+
+// ------------------------------------------------------------------- tiles
+// Head dims that are whole matrix steps. A wave takes 32 keys at a time (16 in
+// f32) for all the row's heads: S^T = K.Q^T with the keys as the matrix rows
+// and the heads as its 16 columns, so a lane holds scores of one head (its
+// column, lane & 15) for keys 4g + r of each 16 (g = lane / 16), and these are,
+// as they lie, the right operand of O^T += V^T.P^T. K goes from memory to the
+// registers of the left operand (16 bytes a lane of a key's row). V^T's
+// operand needs 8 keys of one column a lane: a lane loads its 8 keys' pieces
+// of neighbouring columns and v_perm pairs them up, column after column; the
+// columns then lie in the order lane, element, which the output undoes. No
+// LDS and no barrier until the waves' states meet.
+//
+// Bound by HBM: the matrix steps are 5% of a tile's time at 5 TB/s, whether a
+// row has 1 head or 16. The next tile's rows are loaded before this one's are
+// used; head dims above 128 have no registers for that.
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+template <typename T>
+__device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
+  if constexpr (std::is_same_v<T, f16_t>)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                   0);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same_v<T, f16_t>)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+}
+
+// The larger of the four 16-lane groups' values, on every lane: swapped halves
+// and rows instead of LDS shuffles.
+__device__ __forceinline__ float groups_max(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const float y = fmaxf(__builtin_bit_cast(float, (uint32_t)h[0]), __builtin_bit_cast(float, (uint32_t)h[1]));
+  const uint32_t v = __builtin_bit_cast(uint32_t, y);
+  const auto w = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)w[0]), __builtin_bit_cast(float, (uint32_t)w[1]));
+}
+
+// N dwords at p, which is aligned to an element only.
+template <int N>
+__device__ __forceinline__ void load_words(const void* p, uint32_t* w) {
+  typedef uint32_t words __attribute__((ext_vector_type(N < 2 ? 2 : N)));
+  typedef words unaligned __attribute__((aligned(2)));
+  typedef uint32_t one __attribute__((aligned(2)));
+  if constexpr (N == 1) {
+    w[0] = *static_cast<const one*>(p);
+  } else {
+    const words v = *static_cast<const unaligned*>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = v[i];
+  }
+}
+
+template <typename T, int D>
+struct TileShape {
+  static constexpr bool kHalf = sizeof(T) == 2;
+  static constexpr int kHalves = kHalf ? 2 : 1;             // 16-key halves of a step
+  static constexpr int kKeys = 16 * kHalves;
+  static constexpr int kKWords = D * (int)sizeof(T) / 16;   // dwords of a key's row a lane holds (a quarter)
+  static constexpr int kRows = 4 * kHalves;                 // value rows of a lane
+  static constexpr int kVWords = D * (int)sizeof(T) / 64;   // dwords of a value row a lane holds (a sixteenth)
+  static constexpr int kPieces = kVWords / 4;               // of 4 dwords, then one of the rest
+  static constexpr int kRest = kVWords % 4;
+  static constexpr int kAcc = D / 16;                       // output columns a lane's row of the accumulators holds
+  static constexpr bool kAhead = kHalves * kKWords + kRows * kVWords <= 64;
+};
+
+// One step's keys and values, and which of the lane's keys 16 t + 4g + r are
+// attended (bit 4t + r).
+template <typename T, int D>
+struct Tile {
+  using Sh = TileShape<T, D>;
+  uint32_t k[Sh::kHalves][Sh::kKWords];
+  uint32_t v[Sh::kRows][Sh::kVWords];
+  uint32_t mask;
+};
+
+template <typename T, int D, bool kPage16>
+__device__ __forceinline__ void load_tile(const Shape& s, const Unit& u, const T* __restrict__ k_pages,
+                                          const T* __restrict__ v_pages, const int32_t* __restrict__ table,
+                                          int64_t key0, Tile<T, D>& t) {
+  using Sh = TileShape<T, D>;
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  t.mask = 0;
+#pragma unroll
+  for (int h = 0; h < Sh::kHalves; ++h) {
+    const int64_t key = key0 + 16 * h;
+    int64_t krow, vrow[4];
+    bool ok[4];
+    if constexpr (kPage16) {
+      // 16 keys from a multiple of 16 lie in one page: the same for every lane.
+      const int64_t row = key < u.hi ? row_of(s, table, u.b, u.kv_head, key) : -1;
+      krow = row < 0 ? c : row + c;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        vrow[r] = (row < 0 ? 0 : row) + 4 * g + r;
+        ok[r] = row >= 0;
+      }
+    } else {
+      const int row = (int)row_of(s, table, u.b, u.kv_head, key + c);
+      krow = std::max(row, 0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int x = __shfl(row, 4 * g + r);
+        vrow[r] = std::max(x, 0);
+        ok[r] = x >= 0;
+      }
+    }
+    const T* kr = k_pages + krow * D;
+#pragma unroll
+    for (int i = 0; i < Sh::kKWords / 4; ++i) load_words<4>(kr + (4 * i + g) * (16 / (int)sizeof(T)), t.k[h] + 4 * i);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int64_t j = key + 4 * g + r;
+      if (ok[r] && j >= u.lo && j < u.hi) t.mask |= 1u << (4 * h + r);
+      const T* vr = v_pages + vrow[r] * D;
+      constexpr int E = 16 / (int)sizeof(T);
+#pragma unroll
+      for (int i = 0; i < Sh::kPieces; ++i) load_words<4>(vr + (16 * i + c) * E, t.v[4 * h + r] + 4 * i);
+      if constexpr (Sh::kRest > 0)
+        load_words<Sh::kRest>(vr + 16 * E * Sh::kPieces + c * (Sh::kRest * 4 / (int)sizeof(T)),
+                              t.v[4 * h + r] + 4 * Sh::kPieces);
+    }
+  }
+}
+
+// Output column of accumulator a, matrix row i.
+template <typename T, int D>
+__device__ __forceinline__ int column_of(int a, int i) {
+  using Sh = TileShape<T, D>;
+  constexpr int E = 16 / (int)sizeof(T), R = Sh::kRest * 4 / (int)sizeof(T);
+  return a < Sh::kPieces * E ? (a / E * 16 + i) * E + a % E : Sh::kPieces * 16 * E + i * R + (a - Sh::kPieces * E);
+}
+
+template <typename T, int D>
+struct Heads {
+  uint32_t q[TileShape<T, D>::kKWords];
+  f32x4 o[TileShape<T, D>::kAcc];
+  f32x4 l4;   // 16-bit: the weights' sum, from a matrix step with rows of ones
+  float l;    // f32: this lane's keys' share of it
+  float m;
+  uint32_t seen;
+};
+
+template <typename T, int D>
+__device__ __forceinline__ void use_tile(float scale2, Tile<T, D>& t, Heads<T, D>& st) {
+  using Sh = TileShape<T, D>;
+  f32x4 x[Sh::kHalves];
+#pragma unroll
+  for (int h = 0; h < Sh::kHalves; ++h) {
+    x[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if constexpr (Sh::kHalf) {
+#pragma unroll
+      for (int i = 0; i < Sh::kKWords; i += 4)
+        x[h] = mfma16<T>(u32x4{t.k[h][i], t.k[h][i + 1], t.k[h][i + 2], t.k[h][i + 3]},
+                         u32x4{st.q[i], st.q[i + 1], st.q[i + 2], st.q[i + 3]}, x[h]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < Sh::kKWords; ++i)
+        x[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, t.k[h][i]),
+                                                    __builtin_bit_cast(float, st.q[i]), x[h], 0, 0, 0);
+    }
+  }
+  constexpr uint32_t kAll = (1u << Sh::kRows) - 1;
+  if (__any(t.mask != kAll)) {
+    // What is not attended weighs nothing whatever its rows hold.
+#pragma unroll
+    for (int r = 0; r < Sh::kRows; ++r)
+      if (!(t.mask >> r & 1)) {
+#pragma unroll
+        for (int i = 0; i < Sh::kVWords; ++i) t.v[r][i] = 0;
+      }
+  }
+  st.seen |= t.mask;
+  float mx = -INFINITY;
+#pragma unroll
+  for (int h = 0; h < Sh::kHalves; ++h)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      x[h][r] = t.mask >> (4 * h + r) & 1 ? x[h][r] * scale2 : -INFINITY;
+      mx = fmaxf(mx, x[h][r]);
+    }
+  mx = groups_max(mx);
+  if (__any(mx > st.m)) {
+    const float mn = fmaxf(st.m, mx);
+    const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.m - mn);
+    st.m = mn;
+    st.l *= alpha;
+    st.l4 *= alpha;
+#pragma unroll
+    for (int a = 0; a < Sh::kAcc; ++a) st.o[a] *= alpha;
+  }
+  const float ref = st.m == -INFINITY ? 0.f : st.m;
+#pragma unroll
+  for (int h = 0; h < Sh::kHalves; ++h)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[h][r] = __builtin_amdgcn_exp2f(x[h][r] - ref);
+  if constexpr (Sh::kHalf) {
+    // The weights are rounded to the type for the matrix step, and summed as
+    // rounded, so that a key of all the weight answers its value.
+    const u32x4 p = {pack2<T>(x[0][0], x[0][1]), pack2<T>(x[0][2], x[0][3]), pack2<T>(x[1][0], x[1][1]),
+                     pack2<T>(x[1][2], x[1][3])};
+    constexpr uint32_t one = std::is_same_v<T, f16_t> ? 0x3c003c00u : 0x3f803f80u;
+    st.l4 = mfma16<T>(u32x4{one, one, one, one}, p, st.l4);
+#pragma unroll
+    for (int w = 0; w < Sh::kVWords; ++w)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t sel = e ? 0x07060302u : 0x05040100u;
+        const u32x4 a = {__builtin_amdgcn_perm(t.v[1][w], t.v[0][w], sel), __builtin_amdgcn_perm(t.v[3][w], t.v[2][w], sel),
+                         __builtin_amdgcn_perm(t.v[5][w], t.v[4][w], sel), __builtin_amdgcn_perm(t.v[7][w], t.v[6][w], sel)};
+        st.o[2 * w + e] = mfma16<T>(a, p, st.o[2 * w + e]);
+      }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      st.l += x[0][r];
+#pragma unroll
+      for (int w = 0; w < Sh::kVWords; ++w)
+        st.o[w] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, t.v[r][w]), x[0][r], st.o[w], 0, 0, 0);
+    }
+  }
+}
+
+template <typename T, int D, bool kPage16>
+__global__ void __launch_bounds__(kWaves * 64, D > 192 ? 1 : 2)
+    paged_tiles(Shape s, const T* __restrict__ q, const T* __restrict__ k_pages, const T* __restrict__ v_pages,
+                const int32_t* __restrict__ table, const int32_t* __restrict__ lengths, T* __restrict__ out,
+                float* __restrict__ scratch) {
+  using Sh = TileShape<T, D>;
+  __shared__ float ml[kWaves][kHeads][2];
+  extern __shared__ float ow[];  // [waves][heads][D]
+  Unit u;
+  if (!find_unit(s, lengths, &u)) return;
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Heads<T, D> st;
+  st.m = -INFINITY;
+  st.l = 0.f;
+  st.l4 = f32x4{0.f, 0.f, 0.f, 0.f};
+  st.seen = 0;
+#pragma unroll
+  for (int a = 0; a < Sh::kAcc; ++a) st.o[a] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const T* qr = q + (u.b * s.p.Hq + u.head0 + std::min(c, u.heads - 1)) * D;
+#pragma unroll
+  for (int i = 0; i < Sh::kKWords / 4; ++i) {
+    load_words<4>(qr + (4 * i + g) * (16 / (int)sizeof(T)), st.q + 4 * i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) st.q[4 * i + e] = c < u.heads ? st.q[4 * i + e] : 0u;
+  }
+  const float scale2 = s.p.scale * kLog2e;
+  // Step i of the wave: its tiles are every kWaves-th from tile0 + wave.
+  constexpr int kSteps = kTileKeys / Sh::kKeys;
+  const int steps = u.tile0 + wave < u.tile1 ? ((u.tile1 - u.tile0 - wave + kWaves - 1) / kWaves) * kSteps : 0;
+  auto key_of = [&](int i) {
+    return (int64_t)(u.tile0 + wave + i / kSteps * kWaves) * kTileKeys + i % kSteps * Sh::kKeys;
+  };
+  if (steps > 0) {
+    Tile<T, D> t;
+    if constexpr (Sh::kAhead) {
+      load_tile<T, D, kPage16>(s, u, k_pages, v_pages, table, key_of(0), t);
+      for (int i = 1; i < steps; ++i) {
+        Tile<T, D> next;
+        load_tile<T, D, kPage16>(s, u, k_pages, v_pages, table, key_of(i), next);
+        use_tile<T, D>(scale2, t, st);
+        t = next;
+      }
+      use_tile<T, D>(scale2, t, st);
+    } else {
+      for (int i = 0; i < steps; ++i) {
+        load_tile<T, D, kPage16>(s, u, k_pages, v_pages, table, key_of(i), t);
+        use_tile<T, D>(scale2, t, st);
+      }
+    }
+  }
+  float l = st.l4[0];
+  if constexpr (!Sh::kHalf) l = st.l + __shfl_xor(st.l, 16), l += __shfl_xor(l, 32);
+  const bool any = __any(st.seen != 0);
+  if (lane < u.heads) {
+    ml[wave][lane][0] = st.m;
+    ml[wave][lane][1] = any ? l : -1.f;
+  }
+  if (any && c < u.heads) {
+#pragma unroll
+    for (int a = 0; a < Sh::kAcc; ++a)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) ow[(wave * u.heads + c) * D + column_of<T, D>(a, 4 * g + r)] = st.o[a][r];
+  }
+  __syncthreads();
+  finish_heads<T>(s, u, 0, u.heads, ml, ow, out, scratch);
 }
 
 // One workgroup a query head: folds the splits of its row in split order.
@@ -334,14 +645,37 @@ void launch_paged_attention(hipStream_t stream, const PagedParams& p, DType t, c
   const int64_t rows = p.B * s.rows;
   // Splits of unit_tiles tiles, and one that is short a row.
   const int64_t units = std::min<int64_t>(rows * most_splits(s), rows + kUnits);
+  // The waves' outputs, [waves][heads][D].
+  const size_t lds = static_cast<size_t>(kWaves) * s.heads * p.D * sizeof(float);
   auto go = [&](auto tag) {
     using T = decltype(tag);
-    hipLaunchKernelGGL((paged_any<T>), dim3(static_cast<uint32_t>(units)), dim3(kWaves * 64), 0, stream, s,
-                       static_cast<const T*>(q), static_cast<const T*>(k_pages), static_cast<const T*>(v_pages),
-                       page_table, lengths, static_cast<T*>(out), static_cast<float*>(scratch));
+    const T *qp = static_cast<const T*>(q), *kp = static_cast<const T*>(k_pages), *vp = static_cast<const T*>(v_pages);
+    const dim3 grid(static_cast<uint32_t>(units)), block(kWaves * 64);
+    T* op = static_cast<T*>(out);
+    float* sp = static_cast<float*>(scratch);
+#define PJRTX_PAGED(DIM)                                                                                      \
+  case DIM:                                                                                                   \
+    if (p.S % 16 == 0)                                                                                        \
+      hipLaunchKernelGGL((paged_tiles<T, DIM, true>), grid, block, lds, stream, s, qp, kp, vp, page_table,    \
+                         lengths, op, sp);                                                                    \
+    else                                                                                                      \
+      hipLaunchKernelGGL((paged_tiles<T, DIM, false>), grid, block, lds, stream, s, qp, kp, vp, page_table,   \
+                         lengths, op, sp);                                                                    \
+    break
+    switch (p.D) {
+      PJRTX_PAGED(32);
+      PJRTX_PAGED(64);
+      PJRTX_PAGED(96);
+      PJRTX_PAGED(128);
+      PJRTX_PAGED(192);
+      PJRTX_PAGED(256);
+      default:
+        hipLaunchKernelGGL((paged_any<T>), grid, block, 0, stream, s, qp, kp, vp, page_table, lengths, op, sp);
+    }
+#undef PJRTX_PAGED
     if (scratch)
       hipLaunchKernelGGL((paged_combine<T>), dim3(static_cast<uint32_t>(p.B * p.Hq)), dim3(256), 0, stream, s, lengths,
-                         static_cast<const float*>(scratch), static_cast<T*>(out));
+                         sp, op);
   };
   if (t == DType::kF32) go(float());
   else if (t == DType::kBF16) go(bf16_t());

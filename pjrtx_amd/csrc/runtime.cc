@@ -979,8 +979,9 @@ void Executable::run_step(Loaded* L, size_t si, std::vector<MemRef>& vals, int p
         for (size_t k = 0; k < s.outputs.size(); ++k) {
           auto ww = s.window_out.find(static_cast<int>(k));
           // A fused in-place dynamic_update_slice result is its operand's buffer.
-          vals[s.outputs[k]] = ww != s.window_out.end() ? vals[ww->second.operand]
-                                                        : dev->allocate(prog_.type(s.outputs[k]).bytes());
+          if (ww != s.window_out.end()) vals[s.outputs[k]] = vals[ww->second.operand];
+          else if (placed && (*placed)[s.outputs[k]]) vals[s.outputs[k]] = (*placed)[s.outputs[k]];
+          else vals[s.outputs[k]] = dev->allocate(prog_.type(s.outputs[k]).bytes());
         }
       }
       if (s.kind == StepKind::kLoop && num_elements(s.loop_shape) == 0) return;
@@ -1196,12 +1197,14 @@ size_t Executable::execute_noalloc(Device* dev, const void* const* args, size_t 
   };
   std::vector<MemRef> placed(prog_.values.size());
   for (const Step& st : plan_.steps) {
-    if (st.kind != StepKind::kLibrary || operator_lib_kind(prog_.ops[st.lib_op].kind) == LibKind::kCopy) continue;
+    const bool oper = st.kind == StepKind::kLibrary && operator_lib_kind(prog_.ops[st.lib_op].kind) != LibKind::kCopy;
+    if (!oper && st.kind != StepKind::kLoop) continue;
     for (int v : st.outputs) {
       const auto first = std::find(prog_.results.begin(), prog_.results.end(), v);
       if (first == prog_.results.end() || std::count(first, prog_.results.end(), v) > 1) continue;
       const size_t i = first - prog_.results.begin();
-      if (!alone(i, -1)) continue;
+      // The generated kernels' vector stores take blocks as the arena's.
+      if (!alone(i, -1) || (!oper && reinterpret_cast<uintptr_t>(outs[i]) % 256 != 0)) continue;
       auto m = std::make_shared<DeviceMemory>();
       m->dev = dev;
       m->ptr = outs[i];

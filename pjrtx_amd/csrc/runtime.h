@@ -313,7 +313,8 @@ class Executable {
   // intermediate, copy of a parameter the plan writes, and kernel scratch
   // block comes from the device's fixed no-allocation block (kernels/
   // noalloc.h), whose contents the previous call left behind. A result that
-  // an operator's step produces is written straight to its output, and an
+  // an operator or a generated elementwise kernel produces is written straight
+  // to its output (elementwise: at a multiple of 256 bytes), and an
   // output at the address of the donated argument that the plan writes in
   // place for it (the argument's `tf.aliasing_output`) is written there, where
   // no other argument or output of the call overlaps either. Work is queued
