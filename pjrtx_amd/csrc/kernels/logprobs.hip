@@ -6,9 +6,9 @@
 // x so far m, l = sum e^(x-m), a = sum e^(x-m) (x-m)), from which lse = m +
 // log l and entropy = log l - a / l: the entropy's terms are taken about m,
 // not about zero, so nothing large cancels. Elements that may be among the
-// row's top_k (bounded below by the top_k-th largest of the threads' maxima,
-// then by the best found so far) go to a list in LDS and are ranked there by
-// value, then by lowest index. logprobs_join folds a row's splits in order.
+// row's top_k (bounded below by the threads' maxima, then by the top_k found so
+// far) go to a list in LDS and are ranked there by value, then by lowest index.
+// logprobs_join folds a row's splits.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -22,7 +22,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kChunk = 8192;               // elements a workgroup holds in registers
 constexpr int kCandidates = 1024;          // list of a chunk's candidates in LDS
-constexpr int kJoinKeys = 1024;            // top_k keys of all splits that the join ranks
+constexpr int kJoinKeys = 2048;            // keys of all splits that the join holds in LDS
+constexpr int kJoinSplits = 64;            // a lane each
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // The order of top_k on floats: the sign-magnitude order of their bits, so
@@ -54,19 +55,44 @@ __device__ __forceinline__ Soft join(const Soft& x, const Soft& y) {
   return {m, x.l * fx + y.l * fy, fx * (x.a + dx * x.l) + fy * (y.a + dy * y.l)};
 }
 
-// The split's results: {m, l, a}, then top_k keys, largest first.
+// The split's results: {m, l, a}, then top_k keys, largest first, 0 past the last.
 __host__ __device__ constexpr int64_t split_words(int top_k) { return 4 + 2 * (int64_t)top_k; }
 
-// Ranks the n distinct keys at `keys` and leaves the top_k largest (or n, then
-// zeros) in order at `best`. Called by the whole workgroup.
-__device__ __forceinline__ void rank_keys(const uint64_t* keys, int n, uint64_t* best, int top_k) {
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const uint64_t mine = keys[i];
-    int above = 0;
-    for (int j = 0; j < n; ++j) above += keys[j] > mine ? 1 : 0;
-    if (above < top_k) best[above] = mine;
+// The largest of a wave's values, on every lane (register moves, no LDS).
+__device__ __forceinline__ uint32_t wave_max_u(uint32_t x) {
+  const auto take = [](uint32_t a, int b) { return std::max(a, (uint32_t)b); };
+  x = take(x, __builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false));  // the lane 1 before in its 16
+  x = take(x, __builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false));
+  x = take(x, __builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false));
+  x = take(x, __builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false));
+  x = take(x, __builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false));  // lane 15 of the 16 before
+  x = take(x, __builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false));  // lane 31
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
+// The k-th largest of a wave's values (k >= 1).
+__device__ __forceinline__ uint32_t wave_kth_u(uint32_t x, int k) {
+  uint32_t top = 0;
+  for (int i = 0; i < k; ++i) {
+    top = wave_max_u(x);
+    const uint64_t who = __ballot(x == top);
+    if ((int)(threadIdx.x & 63) == __ffsll((unsigned long long)who) - 1) x = 0;
   }
-  for (int i = n + threadIdx.x; i < top_k; i += kThreads) best[i] = 0;
+  return top;
+}
+
+// Ranks the n distinct keys at `cand` together with the `held` at `best` and
+// leaves the top_k largest in order at `to`. Called by the whole workgroup.
+__device__ __forceinline__ void rank_keys(const uint64_t* cand, int n, const uint64_t* best, int held, uint64_t* to,
+                                          int top_k) {
+  for (int i = threadIdx.x; i < n + held; i += kThreads) {
+    const uint64_t mine = i < n ? cand[i] : best[i - n];
+    int above = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) above += cand[j] > mine ? 1 : 0;
+#pragma unroll 4
+    for (int j = 0; j < held; ++j) above += best[j] > mine ? 1 : 0;
+    if (above < top_k) to[above] = mine;
+  }
 }
 
 __device__ __forceinline__ int64_t read_token(const void* tokens, int bytes, int64_t i) {
@@ -80,24 +106,20 @@ __global__ void __launch_bounds__(kThreads)
                    uint32_t* __restrict__ part) {
   constexpr int E = kVecElems<T>;
   constexpr int NV = kChunk / kThreads / E;
-  __shared__ uint64_t cand[kTop ? kCandidates + kLogprobsMaxTopK : 1];
-  __shared__ uint64_t best[kTop ? kLogprobsMaxTopK : 1];
-  __shared__ uint32_t maxima[kTop ? kThreads : 1];
-  __shared__ uint64_t pick[kTop ? kThreads / 64 : 1];
-  __shared__ uint32_t bound_s;
+  constexpr int kWaves = kThreads / 64;
+  __shared__ uint64_t cand[kTop ? kCandidates : 1];
+  __shared__ uint64_t best[2][kTop ? kLogprobsMaxTopK : 1];
+  __shared__ uint32_t kth[kWaves];
+  __shared__ uint64_t pick[kWaves];
   __shared__ int count_s;
-  __shared__ Soft soft_s[kThreads / 64];
+  __shared__ Soft soft_s[kWaves];
   const int64_t row = blockIdx.x / nsplit;
   const int split = (int)(blockIdx.x % nsplit);
   const T* x = logits + row * p.V;
   const int64_t lo = split * per, hi = std::min(p.V, lo + per);
   const int tid = threadIdx.x;
   Soft s = {-INFINITY, 0.f, 0.f};
-  uint32_t bound = 0;  // elements of a lower order are not among the top_k
-  bool have = false;   // best holds top_k keys of this split
-  if constexpr (kTop) {
-    for (int i = tid; i < p.top_k; i += kThreads) best[i] = 0;
-  }
+  int held = 0, turn = 0;  // keys at best[turn]
   for (int64_t base = lo; base < hi; base += kChunk) {
     typename Vec<T>::type v[NV];
 #pragma unroll
@@ -105,11 +127,20 @@ __global__ void __launch_bounds__(kThreads)
       const int64_t at = base + (int64_t)(i * kThreads + tid) * E;
       v[i] = load_vec<T>(x + std::min(at, p.V - 1), hi - at, (T)-INFINITY);
     }
-    float cm = -INFINITY;
+    float cm = -INFINITY;  // NaN where one is
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int e = 0; e < E; ++e) cm = fmaxf(cm, (float)v[i][e]);
+      for (int e = 0; e < E; ++e) cm = __builtin_elementwise_maximum(cm, (float)v[i][e]);
+    if constexpr (kTop) {
+      // Each of the 4 waves has ceil(top_k / 4) threads whose largest element
+      // is at or above the least of these: top_k elements or more are.
+      if (held < p.top_k) {
+        const uint32_t k = wave_kth_u(order_of(cm), (p.top_k + kWaves - 1) / kWaves);
+        if ((tid & 63) == 0) kth[tid >> 6] = k;
+      }
+      if (tid == 0) count_s = 0;
+    }
     const float m = fmaxf(s.m, cm);
     if (m > s.m) {  // also the first finite chunk, from l = a = 0
       const float d = fmaxf(s.m - m, -1e4f), f = exp2f(d * kLog2e);
@@ -130,54 +161,37 @@ __global__ void __launch_bounds__(kThreads)
       }
     if constexpr (kTop) {
       const int64_t left = hi - base;
-      auto index = [&](int i, int e) { return (int64_t)(i * kThreads + tid) * E + e; };
-      if (!have) {
-        // top_k <= 128 < 256 threads: the top_k-th largest of the threads'
-        // maxima is at or below the top_k-th largest element.
-        uint32_t mine = 0;
+      __syncthreads();
+      // Elements at the bound count in the first chunk; behind top_k keys that
+      // were found before (at lower indices) they do not. NaNs always do.
+      const bool full = held == p.top_k;
+      const float bound = full ? value_of((uint32_t)(best[turn][p.top_k - 1] >> 32))
+                               : value_of(std::min(std::min(kth[0], kth[1]), std::min(kth[2], kth[3])));
+      auto may = [&](float y) { return full ? !(y <= bound) : !(y < bound); };
+      if (may(cm)) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
           for (int e = 0; e < E; ++e)
-            if (index(i, e) < left) mine = std::max(mine, order_of((float)v[i][e]));
-        maxima[tid] = mine;
-        __syncthreads();
-        int above = 0;
-        for (int j = 0; j < kThreads; ++j) above += maxima[j] > mine || (maxima[j] == mine && j < tid) ? 1 : 0;
-        if (above == p.top_k - 1) bound_s = mine;
-        __syncthreads();
-        bound = bound_s;
+            if (may((float)v[i][e])) {
+              const int64_t index = (int64_t)(i * kThreads + tid) * E + e;
+              const int at = index < left ? atomicAdd(&count_s, 1) : kCandidates;
+              if (at < kCandidates) cand[at] = key_of((float)v[i][e], base + index);
+            }
       }
-      if (tid == 0) count_s = 0;
       __syncthreads();
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const uint32_t o = order_of((float)v[i][e]);
-          // With top_k keys in hand their last one's order must be passed, or
-          // met at a lower index: those all came before.
-          if ((have ? o > bound : o >= bound) && index(i, e) < left) {
-            const int at = atomicAdd(&count_s, 1);
-            if (at < kCandidates) cand[at] = key_of((float)v[i][e], base + index(i, e));
-          }
-        }
-      __syncthreads();
-      const int n = count_s;
+      int n = count_s;
       if (n > kCandidates) {
         // Too many equal or ordered elements for the list: the top_k of the
-        // chunk one after another, each the largest key below the last.
+        // chunk one after another, each the largest key below the last (read
+        // again: held in registers for this they would halve the waves).
         uint64_t last = ~0ull;
         for (int k = 0; k < p.top_k; ++k) {
           uint64_t mine = 0;
-#pragma unroll
-          for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-              if (index(i, e) < left) {
-                const uint64_t key = key_of((float)v[i][e], base + index(i, e));
-                if (key < last && key > mine) mine = key;
-              }
+          for (int64_t i = tid; i < std::min<int64_t>(left, kChunk); i += kThreads) {
+            const uint64_t key = key_of((float)x[base + i], base + i);
+            if (key < last && key > mine) mine = key;
+          }
 #pragma unroll
           for (int d = 32; d >= 1; d >>= 1) {
             const uint64_t other = __shfl_xor((unsigned long long)mine, d);
@@ -188,27 +202,15 @@ __global__ void __launch_bounds__(kThreads)
           last = std::max(std::max(pick[0], pick[1]), std::max(pick[2], pick[3]));
           if (tid == 0) cand[k] = last;
           __syncthreads();
-          if (last == 0) break;
         }
+        n = p.top_k;
       }
-      int m_keys = n > kCandidates ? p.top_k : n;
-      if (m_keys > 0) {
-        for (int i = tid; i < p.top_k; i += kThreads) cand[m_keys + i] = best[i];
-        __syncthreads();
-        // Empty places of `best` are equal keys of 0 behind all others.
-        int held = p.top_k;
-        if (best[p.top_k - 1] == 0) {
-          held = 0;
-          for (int i = 0; i < p.top_k; ++i) held += best[i] != 0 ? 1 : 0;
-        }
-        __syncthreads();
-        rank_keys(cand, m_keys + held, best, p.top_k);
+      if (n > 0) {
+        rank_keys(cand, n, best[turn], held, best[turn ^ 1], p.top_k);
+        held = std::min(p.top_k, held + n);
+        turn ^= 1;
         __syncthreads();
       }
-      const uint64_t least = best[p.top_k - 1];
-      have = least != 0;
-      bound = (uint32_t)(least >> 32);
-      __syncthreads();
     }
   }
 #pragma unroll
@@ -224,51 +226,70 @@ __global__ void __launch_bounds__(kThreads)
   }
   if constexpr (kTop) {
     for (int i = tid; i < p.top_k; i += kThreads) {
-      out[4 + 2 * i] = (uint32_t)best[i];
-      out[5 + 2 * i] = (uint32_t)(best[i] >> 32);
+      const uint64_t key = i < held ? best[turn][i] : 0;
+      out[4 + 2 * i] = (uint32_t)key;
+      out[5 + 2 * i] = (uint32_t)(key >> 32);
     }
   }
 }
 
+// One wave a row, a lane a split: the softmax states folded by halves, and the
+// splits' ordered keys merged, the largest of the lanes' next ones at a time.
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(64)
     logprobs_join(LogprobsParams p, int nsplit, const T* __restrict__ logits, const void* __restrict__ tokens,
                   const uint32_t* __restrict__ part, float* __restrict__ logprobs, float* __restrict__ entropy,
                   float* __restrict__ lse_out, float* __restrict__ top_logprobs, int32_t* __restrict__ top_tokens) {
   __shared__ uint64_t keys[kJoinKeys];
-  __shared__ uint64_t best[kLogprobsMaxTopK];
-  __shared__ float lse_s;
-  __shared__ int count_s;
   const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x;
   const int64_t words = split_words(p.top_k);
   const uint32_t* in = part + row * nsplit * words;
-  if (threadIdx.x == 0) {
-    count_s = 0;
-    Soft s = {-INFINITY, 0.f, 0.f};
-    for (int k = 0; k < nsplit; ++k)
-      s = join(s, Soft{__builtin_bit_cast(float, in[k * words]), __builtin_bit_cast(float, in[k * words + 1]),
-                       __builtin_bit_cast(float, in[k * words + 2])});
-    const float log_l = logf(s.l);
-    const float lse = s.m + log_l;
-    const int64_t token = read_token(tokens, p.token_bytes, row);
-    logprobs[row] = token >= 0 && token < p.V ? (float)logits[row * p.V + token] - lse : 0.f;
+  const int64_t token = read_token(tokens, p.token_bytes, row);
+  const bool known = token >= 0 && token < p.V;
+  const float chosen = known ? (float)logits[row * p.V + token] : 0.f;
+  for (int i = lane; i < nsplit * p.top_k; i += 64) {
+    const uint32_t* w = in + (i / p.top_k) * words + 4 + 2 * (i % p.top_k);
+    keys[i] = (uint64_t)w[1] << 32 | w[0];
+  }
+  Soft s = {-INFINITY, 0.f, 0.f};
+  if (lane < nsplit) {
+    const uint32_t* w = in + lane * words;
+    s = {__builtin_bit_cast(float, w[0]), __builtin_bit_cast(float, w[1]), __builtin_bit_cast(float, w[2])};
+  }
+  for (int d = 1; d < nsplit; d <<= 1)
+    s = join(s, Soft{__shfl_xor(s.m, d), __shfl_xor(s.l, d), __shfl_xor(s.a, d)});
+  const float log_l = logf(s.l);
+  const float lse = __shfl(s.m + log_l, 0);
+  if (lane == 0) {
+    logprobs[row] = known ? chosen - lse : 0.f;
     entropy[row] = log_l - s.a / s.l;
     lse_out[row] = lse;
-    lse_s = lse;
   }
   if (p.top_k == 0) return;
   __syncthreads();
-  for (int i = threadIdx.x; i < nsplit * p.top_k; i += kThreads) {
-    const uint32_t* w = in + (i / p.top_k) * words + 4 + 2 * (i % p.top_k);
-    const uint64_t key = (uint64_t)w[1] << 32 | w[0];
-    if (key != 0) keys[atomicAdd(&count_s, 1)] = key;  // distinct: their order does not matter
+  int next = 0;
+  uint64_t mine = lane < nsplit ? keys[lane * p.top_k] : 0;
+  uint64_t found[kLogprobsMaxTopK / 64] = {};  // lane i: the keys of ranks i, i + 64, ...
+  for (int k = 0; k < p.top_k; ++k) {
+    const uint32_t high = wave_max_u((uint32_t)(mine >> 32));
+    const bool tied = (uint32_t)(mine >> 32) == high && mine != 0;
+    const uint32_t low = wave_max_u(tied ? (uint32_t)mine : 0u);
+    const uint64_t key = (uint64_t)high << 32 | low;
+    if (mine == key) {
+      ++next;
+      mine = next < p.top_k ? keys[lane * p.top_k + next] : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < kLogprobsMaxTopK / 64; ++j)
+      if (k == j * 64 + lane) found[j] = key;
   }
-  __syncthreads();
-  rank_keys(keys, count_s, best, p.top_k);
-  __syncthreads();
-  for (int i = threadIdx.x; i < p.top_k; i += kThreads) {
-    top_logprobs[row * p.top_k + i] = value_of((uint32_t)(best[i] >> 32)) - lse_s;
-    top_tokens[row * p.top_k + i] = (int32_t)~(uint32_t)best[i];
+#pragma unroll
+  for (int j = 0; j < kLogprobsMaxTopK / 64; ++j) {
+    const int i = j * 64 + lane;
+    if (i >= p.top_k) continue;
+    top_logprobs[row * p.top_k + i] = value_of((uint32_t)(found[j] >> 32)) - lse;
+    top_tokens[row * p.top_k + i] = (int32_t)~(uint32_t)found[j];
   }
 }
 
@@ -322,7 +343,7 @@ struct Split {
 Split split_of(const LogprobsParams& p) {
   const int64_t chunks = (p.V + kChunk - 1) / kChunk;
   int64_t want = std::max<int64_t>(1, (1024 + p.rows - 1) / std::max<int64_t>(1, p.rows));
-  want = std::min<int64_t>(want, p.top_k ? kJoinKeys / p.top_k : 64);
+  want = std::min<int64_t>(want, p.top_k ? std::min(kJoinSplits, kJoinKeys / p.top_k) : kJoinSplits);
   const int64_t n = std::max<int64_t>(1, std::min(chunks, want));
   const int64_t per = (chunks + n - 1) / n * kChunk;
   return {static_cast<int>((p.V + per - 1) / per), per};
@@ -344,14 +365,14 @@ void launch_token_logprobs(hipStream_t s, const LogprobsParams& p, DType t, cons
                            void* scratch) {
   if (p.rows == 0) return;
   const Split sp = split_of(p);
-  const dim3 grid(static_cast<uint32_t>(p.rows * sp.n)), rows(static_cast<uint32_t>(p.rows)), block(kThreads);
+  const dim3 grid(static_cast<uint32_t>(p.rows * sp.n)), block(kThreads);
   uint32_t* part = static_cast<uint32_t*>(scratch);
   auto go = [&](auto tag) {
     using T = decltype(tag);
     const T* x = static_cast<const T*>(logits);
     if (p.top_k) hipLaunchKernelGGL((logprobs_split<T, true>), grid, block, 0, s, p, sp.n, sp.per, x, part);
     else hipLaunchKernelGGL((logprobs_split<T, false>), grid, block, 0, s, p, sp.n, sp.per, x, part);
-    hipLaunchKernelGGL((logprobs_join<T>), rows, block, 0, s, p, sp.n, x, tokens, part, logprobs, entropy, lse,
+    hipLaunchKernelGGL((logprobs_join<T>), dim3(static_cast<uint32_t>(p.rows)), dim3(64), 0, s, p, sp.n, x, tokens, part, logprobs, entropy, lse,
                        top_logprobs, top_tokens);
   };
   if (t == DType::kF32) go(float());
