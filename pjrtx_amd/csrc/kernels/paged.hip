@@ -1,17 +1,21 @@
 // Attention of one new token a sequence over a paged key-value cache, and the
 // rows that are written into its pages.
 //
-// Work units. A row is one sequence with one key-value head and up to 16 of
-// the query heads that share it, so that keys and values are read once for
-// them. The host knows the table's capacity but no length, so the device cuts
-// the work: every workgroup adds the sequences' 32-key tiles (`lengths` is one
-// short read, most of it from L2) and takes unit blockIdx.x of rows x splits,
-// where a split is `unit_tiles` tiles: about kUnits splits in all, of one size
-// whatever the lengths are. A table far larger than its sequences costs
-// nothing, and a long sequence among short ones is cut finer than they are.
+// Work. A row is one sequence with one key-value head and up to 16 of the
+// query heads that share it, so that keys and values are read once for them.
+// The host knows the table's capacity but no length, so the device cuts the
+// work: every workgroup adds the sequences' 32-key tiles (`lengths` is one
+// short read, most of it from L2), and takes its equal share of the rows' tiles
+// laid end to end: the end of one row, whole ones, the start of another. All
+// workgroups of a launch are resident at once and end together whatever the
+// lengths are; a table far larger than its sequences costs nothing. (64 rows of
+// 32 to 4064 keys by 8 heads, 538 MB: splits of rows, each a workgroup, left
+// the last ones alone on the chip, 113 us at best; shares take 100.) Where the
+// table itself is so small that shares are one tile a wave, rows start on a
+// workgroup's first tile instead, so that no workgroup walks two.
 //
-// A split of a row that has several writes its softmax's (max, sum,
-// unnormalised output) to scratch; paged_combine folds them in split order.
+// A share of a row that is not all of it writes its softmax's (max, sum,
+// unnormalised output) to scratch; paged_combine folds them in order.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -23,10 +27,25 @@ namespace pjrtx {
 namespace {
 
 constexpr int kTileKeys = 32;
-constexpr int kUnits = 512;      // splits aimed at: two workgroups a CU
 constexpr int kHeads = 16;       // query heads of a row
+constexpr int kRowCost = 4;      // tiles; 0 / 2 / 4 / 8: 115 / 106 / 101 / 102 us at those 64 sequences
+constexpr int kCus = 256;
+constexpr int kMaxParts = 2 * kCus;  // of a row: at most one a workgroup
 constexpr int kWaves = 4;
 constexpr float kLog2e = 1.44269504088896340736f;
+
+// n / d for n < 2^31 by a multiplication (Granlund and Montgomery, 1994).
+struct Divisor {
+  uint32_t d = 1, m = 0, s = 0;
+};
+Divisor divisor_of(uint32_t d) {
+  Divisor v;
+  v.d = d;
+  while (v.s < 31 && (1u << v.s) < d) ++v.s;
+  v.m = static_cast<uint32_t>(((uint64_t(1) << 32) * ((uint64_t(1) << v.s) - d)) / d + 1);
+  return v;
+}
+__device__ __forceinline__ uint32_t quotient(uint32_t n, const Divisor& v) { return (__umulhi(n, v.m) + n) >> v.s; }
 
 // What the kernels are given beside the tensors.
 struct Shape {
@@ -35,18 +54,26 @@ struct Shape {
   int head_tiles;  // rows of a (sequence, key-value head)
   int heads;       // query heads of a row at most
   int rows;        // rows of a sequence: Hkv * head_tiles
-  int64_t cap;     // keys the table holds
+  uint32_t cap;    // keys the table holds, below 2^31
+  Divisor page;    // keys of a page
+  int groups;      // workgroups of the launch
+  bool aligned;    // rows start on a workgroup's first tile,
+  int each;        // and have so many workgroups
 };
 
 struct Sequence {
-  int64_t lo, hi;  // attended keys
+  uint32_t lo, hi;  // attended keys
   int tile0, tiles;
 };
 __device__ __forceinline__ Sequence sequence_of(const Shape& s, const int32_t* lengths, int64_t b) {
   Sequence q;
-  q.hi = std::min<int64_t>(std::max(lengths[b], 0), s.cap);
-  q.lo = s.p.window > 0 ? std::max<int64_t>(0, q.hi - s.p.window) : 0;
-  q.tile0 = (int)(q.lo / kTileKeys);
+  q.hi = std::min((uint32_t)std::max(lengths[b], 0), s.cap);
+  q.lo = 0;
+  q.tile0 = 0;  // known before the length is, where there is no window
+  if (s.p.window > 0 && s.p.window < q.hi) {
+    q.lo = q.hi - (uint32_t)s.p.window;
+    q.tile0 = (int)(q.lo / kTileKeys);
+  }
   q.tiles = (int)((q.hi + kTileKeys - 1) / kTileKeys) - q.tile0;
   return q;
 }
@@ -57,116 +84,147 @@ __device__ __forceinline__ uint32_t wave_sum_u(uint32_t x) {
   return x;
 }
 
-// Tiles of a split: whole rounds of the workgroup's waves.
-__device__ __forceinline__ uint32_t unit_tiles(const Shape& s, const int32_t* lengths) {
+// Tiles that a row counts for in the rows laid end to end: its own, at least
+// one, so that some workgroup answers for it; then kRowCost for the time that a
+// workgroup takes to begin it.
+__device__ __forceinline__ uint32_t span_of(int tiles) { return (uint32_t)std::max(tiles, 1) + kRowCost; }
+// Tiles of a workgroup's share.
+__device__ __forceinline__ uint32_t share_of(const Shape& s, const int32_t* lengths) {
   uint32_t total = 0;
 #pragma unroll 4
-  for (int64_t b = threadIdx.x & 63; b < s.p.B; b += 64) total += (uint32_t)sequence_of(s, lengths, b).tiles;
-  total = wave_sum_u(total);
-  const uint64_t per = ((uint64_t)total * s.rows + kUnits - 1) / kUnits;
-  return (uint32_t)std::max<uint64_t>(kWaves, (per + kWaves - 1) / kWaves * kWaves);
-}
-__device__ __forceinline__ uint32_t splits_of(int tiles, uint32_t per) {
-  return tiles <= (int)per ? 1u : ((uint32_t)tiles + per - 1) / per;
+  for (int64_t b = threadIdx.x & 63; b < s.p.B; b += 64) total += span_of(sequence_of(s, lengths, b).tiles);
+  total = wave_sum_u(total) * (uint32_t)s.rows;
+  return std::max<uint32_t>(kWaves, (total + s.groups - 1) / s.groups);
 }
 
-// Where a sequence stands in the order of units and of scratch slots: those of
-// the sequences before it, in splits. `slots` counts those with several only.
-struct Place {
-  int64_t b;
-  uint32_t before, slots, n;
-};
-// The sequence that holds split index `at` of the sequences' splits laid end
-// to end, or (kByB) sequence `at` itself. Each wave of the workgroup finds it
-// alone; false past the last.
-template <bool kByB>
-__device__ __forceinline__ bool find_place(const Shape& s, const int32_t* lengths, uint32_t per, uint32_t at,
-                                           Place* out) {
+// The sequence whose rows hold tile `at` of all rows', and the tiles before it.
+// Each wave of the workgroup finds it alone; false past the last.
+__device__ __forceinline__ bool find_sequence(const Shape& s, const int32_t* lengths, uint32_t at, int64_t* b_out,
+                                              uint32_t* before_out) {
   const int lane = threadIdx.x & 63;
-  uint32_t before = 0, slots = 0;
+  uint32_t before = 0;
   for (int64_t b0 = 0; b0 < s.p.B; b0 += 64) {
     const int64_t b = b0 + lane;
-    const uint32_t n = b < s.p.B ? splits_of(sequence_of(s, lengths, b).tiles, per) : 0u;
-    const uint32_t k = n > 1 ? n : 0u;
-    uint32_t sum = n, ksum = k;  // inclusive over the lanes
+    const uint32_t n = b < s.p.B ? span_of(sequence_of(s, lengths, b).tiles) * (uint32_t)s.rows : 0u;
+    uint32_t sum = n;  // inclusive over the lanes
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t a = __shfl_up(sum, d), c = __shfl_up(ksum, d);
-      if (lane >= d) {
-        sum += a;
-        ksum += c;
-      }
+      const uint32_t a = __shfl_up(sum, d);
+      if (lane >= d) sum += a;
     }
     const uint32_t first = before + sum - n;
-    const bool mine = kByB ? b == (int64_t)at : at >= first && at < first + n;
-    const uint64_t who = __ballot(mine);
+    const uint64_t who = __ballot(at >= first && at < first + n);
     if (who) {
       const int src = __ffsll((unsigned long long)who) - 1;
-      out->b = b0 + src;
-      out->before = __shfl(first, src);
-      out->slots = __shfl(slots + ksum - k, src);
-      out->n = __shfl(n, src);
+      *b_out = b0 + src;
+      *before_out = (uint32_t)__builtin_amdgcn_readlane((int)first, src);
       return true;
     }
-    before += __shfl(sum, 63);
-    slots += __shfl(ksum, 63);
+    before += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
   }
   return false;
 }
 
-struct Unit {
-  int64_t b;
-  int kv_head, head0, heads;  // query heads head0 .. head0 + heads - 1
-  uint32_t split, n;
-  int64_t slot;               // scratch slot (n > 1)
-  int64_t lo, hi;             // the sequence's attended keys
-  int tile0, tile1;           // the split's tiles
-};
-__device__ __forceinline__ bool find_unit(const Shape& s, const int32_t* lengths, Unit* u) {
-  const uint32_t per = unit_tiles(s, lengths);
-  const uint32_t r = blockIdx.x % (uint32_t)s.rows;
-  Place pl;
-  if (!find_place<false>(s, lengths, per, blockIdx.x / (uint32_t)s.rows, &pl)) return false;
-  const Sequence q = sequence_of(s, lengths, pl.b);
-  u->b = pl.b;
-  u->kv_head = (int)r / s.head_tiles;
-  const int ht = (int)r % s.head_tiles;
-  u->head0 = u->kv_head * s.group + ht * kHeads;
-  u->heads = std::min(kHeads, s.group - ht * kHeads);
-  u->split = blockIdx.x / (uint32_t)s.rows - pl.before;
-  u->n = pl.n;
-  u->slot = (int64_t)pl.slots * s.rows + (int64_t)r * pl.n + u->split;
-  u->lo = q.lo;
-  u->hi = q.hi;
-  u->tile0 = q.tile0 + (int)(u->split * per);
-  u->tile1 = std::min(q.tile0 + q.tiles, u->tile0 + (int)per);
-  return true;
-}
-
 // Key j's row of the pages (in rows of D elements), -1 where the table's entry
-// names no page. j is clamped to the table.
-__device__ __forceinline__ int64_t row_of(const Shape& s, const int32_t* table, int64_t b, int kv_head, int64_t j) {
-  const int64_t e = std::min(j / s.p.S, s.p.M - 1);
-  const int64_t page = table[b * s.p.M + e];
+// names no page. j is clamped to the table; the pages have fewer than 2^31 rows.
+__device__ __forceinline__ int row_of(const Shape& s, const int32_t* table, int64_t b, int kv_head, uint32_t j) {
+  const uint32_t e = std::min(quotient(j, s.page), (uint32_t)s.p.M - 1);
+  const int page = table[b * s.p.M + e];
   if (page < 0 || page >= s.p.P) return -1;
-  return (page * s.p.Hkv + kv_head) * s.p.S + (j - e * s.p.S);
+  return (page * s.p.Hkv + kv_head) * (int)s.page.d + (int)(j - e * s.page.d);
 }
 
+// What the workgroup that starts a row leaves for paged_combine, before the
+// slots: the row's parts are that workgroup's and the n - 1 after it.
+struct Row {
+  uint32_t group, n;
+};
+// A workgroup has a slot for the end of a row that others start, and one for
+// the start of a row.
+__host__ __device__ constexpr int64_t slot_of(int64_t group, bool start) { return 2 * group + (start ? 1 : 0); }
 // Scratch of a slot: (max, sum) of each head, then each head's D outputs. A
 // sum of -1 marks a split without any attended key.
 __device__ __forceinline__ float* slot_state(const Shape& s, float* scratch, int64_t slot) {
-  return scratch + slot * s.heads * (s.p.D + 2);
+  return scratch + 2 * s.p.B * s.rows + slot * s.heads * (s.p.D + 2);
+}
+
+// The part of a row that a workgroup is at.
+struct Unit {
+  int64_t b;
+  int kv_head, head0, heads;  // query heads head0 .. head0 + heads - 1
+  bool whole;                 // all of the row
+  int64_t slot;               // scratch slot otherwise
+  uint32_t lo, hi;            // the sequence's attended keys
+  int tile0, tile1;           // the part's tiles
+};
+
+__device__ __forceinline__ void set_unit(const Shape& s, Unit* u, uint32_t r, const Sequence& q, uint32_t tile,
+                                         uint32_t n) {
+  const int ht = (int)r % s.head_tiles;
+  u->kv_head = (int)r / s.head_tiles;
+  u->head0 = u->kv_head * s.group + ht * kHeads;
+  u->heads = std::min(kHeads, s.group - ht * kHeads);
+  u->whole = tile == 0 && (int)n >= q.tiles;
+  u->slot = slot_of(blockIdx.x, tile == 0);
+  u->lo = q.lo;
+  u->hi = q.hi;
+  u->tile0 = q.tile0 + (int)tile;
+  u->tile1 = q.tile0 + std::min(q.tiles, (int)(tile + n));
+}
+
+// Calls part(unit) for each part of the workgroup's share, the same on every
+// thread.
+template <bool kAligned, typename F>
+__device__ __forceinline__ void for_parts(const Shape& s, const int32_t* lengths, float* scratch, const F& part) {
+  Unit u;
+  Row* rows = reinterpret_cast<Row*>(scratch);
+  if constexpr (kAligned) {
+    // Row by row, as many workgroups each as the table's keys could take.
+    const uint32_t row = blockIdx.x / (uint32_t)s.each, tile = (blockIdx.x - row * (uint32_t)s.each) * kWaves;
+    u.b = row / (uint32_t)s.rows;
+    const Sequence q = sequence_of(s, lengths, u.b);
+    if (tile > 0 && (int)tile >= q.tiles) return;
+    set_unit(s, &u, row - (uint32_t)u.b * s.rows, q, tile, kWaves);
+    if (rows && tile == 0 && threadIdx.x == 0) rows[row] = {blockIdx.x, ((uint32_t)q.tiles + kWaves - 1) / kWaves};
+    part(u);
+  } else {
+    const uint32_t per = share_of(s, lengths);
+    uint32_t at = blockIdx.x * per, before;
+    if (!find_sequence(s, lengths, at, &u.b, &before)) return;
+    const uint32_t end = at + per;
+    Sequence q = sequence_of(s, lengths, u.b);
+    uint32_t span = span_of(q.tiles);
+    uint32_t r = (at - before) / span, tile = (at - before) % span;
+    for (;;) {
+      const uint32_t own = (uint32_t)std::max(q.tiles, 1);
+      const uint32_t n = std::min(end - at, span - tile);
+      set_unit(s, &u, r, q, tile, n);
+      if (tile == 0 && threadIdx.x == 0)
+        rows[u.b * s.rows + r] = {blockIdx.x, (at + own - 1) / per - blockIdx.x + 1};
+      if (tile < own) part(u);
+      at += n;
+      if (at >= end) return;
+      tile = 0;
+      if (++r == (uint32_t)s.rows) {
+        r = 0;
+        if (++u.b >= s.p.B) return;
+        q = sequence_of(s, lengths, u.b);
+        span = span_of(q.tiles);
+      }
+      __syncthreads();  // the part before has been read from LDS
+    }
+  }
 }
 
 // The workgroup's waves meet: the state of head h in wave w is ml[w][h], a sum
 // of -1 where the wave attended no key, and its outputs are o[(w heads + h) D].
-// Writes the rows' results, or the split's partial ones, of the unit's heads
+// Writes the row's results, or the part's, of the unit's heads
 // first .. first + heads - 1.
 template <typename T>
 __device__ __forceinline__ void finish_heads(const Shape& s, const Unit& u, int first, int heads,
                                              const float (*ml)[kHeads][2], const float* o, T* out, float* scratch) {
   const int D = s.p.D;
-  float* state = u.n > 1 ? slot_state(s, scratch, u.slot) : nullptr;
+  float* state = u.whole ? nullptr : slot_state(s, scratch, u.slot);
   for (int i = threadIdx.x; i < heads * D; i += kWaves * 64) {
     const int h = i / D, d = i - h * D, hu = first + h;
     float m = -INFINITY;
@@ -202,15 +260,11 @@ __device__ __forceinline__ void finish_heads(const Shape& s, const Unit& u, int 
 // lanes across the head dim, one query head after another.
 constexpr int kMaxHeadDim = 512;
 template <typename T>
-__global__ void __launch_bounds__(kWaves * 64)
-    paged_any(Shape s, const T* __restrict__ q, const T* __restrict__ k_pages, const T* __restrict__ v_pages,
-              const int32_t* __restrict__ table, const int32_t* __restrict__ lengths, T* __restrict__ out,
-              float* __restrict__ scratch) {
+__device__ __forceinline__ void any_part(const Shape& s, const Unit& u, const T* __restrict__ q,
+                                         const T* __restrict__ k_pages, const T* __restrict__ v_pages,
+                                         const int32_t* __restrict__ table, T* __restrict__ out, float* scratch,
+                                         float (*ml)[kHeads][2], float* ow) {
   constexpr int J = kMaxHeadDim / 64;
-  __shared__ float ml[kWaves][kHeads][2];
-  __shared__ float ow[kWaves * kMaxHeadDim];  // [waves][D]
-  Unit u;
-  if (!find_unit(s, lengths, &u)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int D = s.p.D;
   for (int h = 0; h < u.heads; ++h) {
@@ -223,12 +277,12 @@ __global__ void __launch_bounds__(kWaves * 64)
     }
     float m = -INFINITY, l = -1.f;
     for (int t = u.tile0 + wave; t < u.tile1; t += kWaves) {
-      const int64_t first = std::max<int64_t>(u.lo, (int64_t)t * kTileKeys);
-      const int64_t last = std::min<int64_t>(u.hi, ((int64_t)t + 1) * kTileKeys);
-      for (int64_t key = first; key < last; ++key) {
-        const int64_t row = row_of(s, table, u.b, u.kv_head, key);
+      const uint32_t first = std::max(u.lo, (uint32_t)t * kTileKeys);
+      const uint32_t last = std::min(u.hi, ((uint32_t)t + 1) * kTileKeys);
+      for (uint32_t key = first; key < last; ++key) {
+        const int row = row_of(s, table, u.b, u.kv_head, key);
         if (row < 0) continue;
-        const T *kr = k_pages + row * D, *vr = v_pages + row * D;
+        const T *kr = k_pages + (int64_t)row * D, *vr = v_pages + (int64_t)row * D;
         float dot = 0.f, vv[J];
 #pragma unroll
         for (int j = 0; j < J; ++j) {
@@ -258,6 +312,17 @@ __global__ void __launch_bounds__(kWaves * 64)
     finish_heads<T>(s, u, h, 1, ml, ow, out, scratch);
     __syncthreads();
   }
+}
+
+template <typename T, bool kAligned>
+__global__ void __launch_bounds__(kWaves * 64)
+    paged_any(Shape s, const T* __restrict__ q, const T* __restrict__ k_pages, const T* __restrict__ v_pages,
+              const int32_t* __restrict__ table, const int32_t* __restrict__ lengths, T* __restrict__ out,
+              float* __restrict__ scratch) {
+  __shared__ float ml[kWaves][kHeads][2];
+  __shared__ float ow[kWaves * kMaxHeadDim];  // [waves][D]
+  for_parts<kAligned>(s, lengths, scratch,
+            [&](const Unit& u) { any_part<T>(s, u, q, k_pages, v_pages, table, out, scratch, ml, ow); });
 }
 
 // ------------------------------------------------------------------- tiles
@@ -353,18 +418,18 @@ struct Tile {
 template <typename T, int D, bool kPage16>
 __device__ __forceinline__ void load_tile(const Shape& s, const Unit& u, const T* __restrict__ k_pages,
                                           const T* __restrict__ v_pages, const int32_t* __restrict__ table,
-                                          int64_t key0, Tile<T, D>& t) {
+                                          uint32_t key0, Tile<T, D>& t) {
   using Sh = TileShape<T, D>;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   t.mask = 0;
 #pragma unroll
   for (int h = 0; h < Sh::kHalves; ++h) {
-    const int64_t key = key0 + 16 * h;
-    int64_t krow, vrow[4];
+    const uint32_t key = key0 + 16 * h;
+    int krow, vrow[4];
     bool ok[4];
     if constexpr (kPage16) {
       // 16 keys from a multiple of 16 lie in one page: the same for every lane.
-      const int64_t row = key < u.hi ? row_of(s, table, u.b, u.kv_head, key) : -1;
+      const int row = row_of(s, table, u.b, u.kv_head, key);
       krow = row < 0 ? c : row + c;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -372,7 +437,7 @@ __device__ __forceinline__ void load_tile(const Shape& s, const Unit& u, const T
         ok[r] = row >= 0;
       }
     } else {
-      const int row = (int)row_of(s, table, u.b, u.kv_head, key + c);
+      const int row = row_of(s, table, u.b, u.kv_head, key + c);
       krow = std::max(row, 0);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -381,14 +446,14 @@ __device__ __forceinline__ void load_tile(const Shape& s, const Unit& u, const T
         ok[r] = x >= 0;
       }
     }
-    const T* kr = k_pages + krow * D;
+    const T* kr = k_pages + (int64_t)krow * D;
 #pragma unroll
     for (int i = 0; i < Sh::kKWords / 4; ++i) load_words<4>(kr + (4 * i + g) * (16 / (int)sizeof(T)), t.k[h] + 4 * i);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int64_t j = key + 4 * g + r;
+      const uint32_t j = key + 4 * g + r;
       if (ok[r] && j >= u.lo && j < u.hi) t.mask |= 1u << (4 * h + r);
-      const T* vr = v_pages + vrow[r] * D;
+      const T* vr = v_pages + (int64_t)vrow[r] * D;
       constexpr int E = 16 / (int)sizeof(T);
 #pragma unroll
       for (int i = 0; i < Sh::kPieces; ++i) load_words<4>(vr + (16 * i + c) * E, t.v[4 * h + r] + 4 * i);
@@ -498,15 +563,11 @@ __device__ __forceinline__ void use_tile(float scale2, Tile<T, D>& t, Heads<T, D
 }
 
 template <typename T, int D, bool kPage16>
-__global__ void __launch_bounds__(kWaves * 64, D > 192 ? 1 : 2)
-    paged_tiles(Shape s, const T* __restrict__ q, const T* __restrict__ k_pages, const T* __restrict__ v_pages,
-                const int32_t* __restrict__ table, const int32_t* __restrict__ lengths, T* __restrict__ out,
-                float* __restrict__ scratch) {
+__device__ __forceinline__ void tiles_part(const Shape& s, const Unit& u, const T* __restrict__ q,
+                                           const T* __restrict__ k_pages, const T* __restrict__ v_pages,
+                                           const int32_t* __restrict__ table, T* __restrict__ out, float* scratch,
+                                           float (*ml)[kHeads][2], float* ow) {
   using Sh = TileShape<T, D>;
-  __shared__ float ml[kWaves][kHeads][2];
-  extern __shared__ float ow[];  // [waves][heads][D]
-  Unit u;
-  if (!find_unit(s, lengths, &u)) return;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Heads<T, D> st;
@@ -528,7 +589,7 @@ __global__ void __launch_bounds__(kWaves * 64, D > 192 ? 1 : 2)
   constexpr int kSteps = kTileKeys / Sh::kKeys;
   const int steps = u.tile0 + wave < u.tile1 ? ((u.tile1 - u.tile0 - wave + kWaves - 1) / kWaves) * kSteps : 0;
   auto key_of = [&](int i) {
-    return (int64_t)(u.tile0 + wave + i / kSteps * kWaves) * kTileKeys + i % kSteps * Sh::kKeys;
+    return (uint32_t)(u.tile0 + wave + i / kSteps * kWaves) * kTileKeys + i % kSteps * Sh::kKeys;
   };
   if (steps > 0) {
     Tile<T, D> t;
@@ -565,45 +626,100 @@ __global__ void __launch_bounds__(kWaves * 64, D > 192 ? 1 : 2)
   finish_heads<T>(s, u, 0, u.heads, ml, ow, out, scratch);
 }
 
-// One workgroup a query head: folds the splits of its row in split order.
-template <typename T>
+template <typename T, int D, bool kPage16, bool kAligned>
+__global__ void __launch_bounds__(kWaves * 64, D > 192 ? 1 : 2)
+    paged_tiles(Shape s, const T* __restrict__ q, const T* __restrict__ k_pages, const T* __restrict__ v_pages,
+                const int32_t* __restrict__ table, const int32_t* __restrict__ lengths, T* __restrict__ out,
+                float* __restrict__ scratch) {
+  __shared__ float ml[kWaves][kHeads][2];
+  extern __shared__ float ow[];  // [waves][heads][D]
+  for_parts<kAligned>(s, lengths, scratch, [&](const Unit& u) {
+    tiles_part<T, D, kPage16>(s, u, q, k_pages, v_pages, table, out, scratch, ml, ow);
+  });
+}
+
+// One workgroup a query head: folds the parts of its row. Lanes take V outputs
+// each, groups of them every G-th part, and the groups are added in order.
+template <typename T, int V>
 __global__ void __launch_bounds__(256)
-    paged_combine(Shape s, const int32_t* __restrict__ lengths, const float* __restrict__ scratch,
-                  T* __restrict__ out) {
-  __shared__ float m_s[kUnits + 1], l_s[kUnits + 1];
+    paged_combine(Shape s, const float* __restrict__ scratch, T* __restrict__ out) {
+  __shared__ float f_s[kMaxParts], l_s[kMaxParts];
+  __shared__ float red[2][4];
+  __shared__ float sums[256 * V];
   const int64_t b = blockIdx.x / s.p.Hq;
   const int hq = (int)(blockIdx.x % s.p.Hq);
-  const uint32_t per = unit_tiles(s, lengths);
-  Place pl;
-  if (!find_place<true>(s, lengths, per, (uint32_t)b, &pl) || pl.n <= 1) return;
   const int kv_head = hq / s.group, ht = (hq % s.group) / kHeads, head = (hq % s.group) % kHeads;
-  const int64_t slot0 = (int64_t)pl.slots * s.rows + (int64_t)(kv_head * s.head_tiles + ht) * pl.n;
-  const int64_t words = (int64_t)s.heads * (s.p.D + 2);
-  const float* base = scratch + slot0 * words;
-  for (uint32_t i = threadIdx.x; i < pl.n; i += 256) {
-    m_s[i] = base[i * words + 2 * head];
-    l_s[i] = base[i * words + 2 * head + 1];
-  }
-  __syncthreads();
+  const Row row = reinterpret_cast<const Row*>(scratch)[b * s.rows + kv_head * s.head_tiles + ht];
+  if (row.n <= 1) return;
+  const int n = (int)row.n, D = s.p.D;
+  // Part i's slot: the first starts the row, the others continue it.
+  auto part = [&](int i) {
+    return slot_state(s, const_cast<float*>(scratch), slot_of((int64_t)row.group + i, i == 0));
+  };
+  // The thread's first outputs are requested with the states.
+  const int lanes = std::min(256, (D + V - 1) / V), groups = 256 / lanes;
+  const int g = threadIdx.x / lanes, lane = threadIdx.x % lanes;
+  float first[V];
+  if (g < std::min(groups, n) && lane * V < D)
+    __builtin_memcpy(first, part(g) + 2 * s.heads + (int64_t)head * D + lane * V, sizeof(first));
   float m = -INFINITY;
-  bool any = false;
-  for (uint32_t i = 0; i < pl.n; ++i) {
-    if (l_s[i] < 0.f) continue;
-    any = true;
-    m = fmaxf(m, m_s[i]);
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const float* state = part(i) + 2 * head;
+    f_s[i] = state[0];
+    l_s[i] = state[1];
+    if (!(l_s[i] < 0.f)) m = fmaxf(m, f_s[i]);
   }
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+  if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   const float ref = m == -INFINITY ? 0.f : m;
-  for (int d = threadIdx.x; d < s.p.D; d += 256) {
-    float l = 0.f, v = 0.f;
-    for (uint32_t i = 0; i < pl.n; ++i) {
-      if (l_s[i] < 0.f) continue;
-      const float f = exp2f(m_s[i] - ref);
-      l += l_s[i] * f;
-      v += f * base[i * words + 2 * s.heads + (int64_t)head * s.p.D + d];
+  // Each part's weight, once; a part without any attended key (a sum of -1)
+  // has no outputs, and weighs -1.
+  float l = 0.f;
+  bool any = false;
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const bool none = l_s[i] < 0.f;
+    f_s[i] = none ? -1.f : exp2f(f_s[i] - ref);
+    l += none ? 0.f : l_s[i] * f_s[i];
+    any = any || !none;
+  }
+  l = wave_sum(l);
+  if ((threadIdx.x & 63) == 0) red[1][threadIdx.x >> 6] = l;
+  any = __syncthreads_or(any);
+  l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  for (int d0 = 0; d0 < D; d0 += lanes * V) {
+    const int d = d0 + lane * V;
+    float acc[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = 0.f;
+    if (g < groups && d < D) {
+#pragma unroll 4
+      for (int i = g; i < n; i += groups) {
+        float x[V];
+        if (i == g && d0 == 0) __builtin_memcpy(x, first, sizeof(x));
+        else __builtin_memcpy(x, part(i) + 2 * s.heads + (int64_t)head * D + d, sizeof(x));
+        const float f = f_s[i];
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] += f < 0.f ? 0.f : x[e] * f;
+      }
     }
-    out[(b * s.p.Hq + hq) * s.p.D + d] = (T)(any ? v / l : 0.f);
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < V; ++e) sums[threadIdx.x * V + e] = acc[e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < lanes * V && d0 + i < D; i += 256) {
+      float v = 0.f;
+      for (int k = 0; k < groups; ++k) v += sums[k * lanes * V + i];
+      out[(b * s.p.Hq + hq) * D + d0 + i] = (T)(any ? v / l : 0.f);
+    }
   }
 }
+
+// Workgroups a CU holds of the kernel that takes the shape: what its registers
+// leave, so that a launch's workgroups run at once.
+int groups_per_cu(const PagedParams& p) { return p.D > 192 ? 1 : 2; }
 
 Shape shape_of(const PagedParams& p) {
   Shape s;
@@ -612,14 +728,19 @@ Shape shape_of(const PagedParams& p) {
   s.head_tiles = (s.group + kHeads - 1) / kHeads;
   s.heads = std::min(s.group, kHeads);
   s.rows = p.Hkv * s.head_tiles;
-  s.cap = p.M * p.S;
+  s.cap = static_cast<uint32_t>(p.M * p.S);
+  s.page = divisor_of(static_cast<uint32_t>(p.S));
+  // The table's tiles as workgroups of one tile a wave, row by row: where they
+  // are no more than run at once, that is the launch.
+  const int64_t tiles = (static_cast<int64_t>(s.cap) + kTileKeys - 1) / kTileKeys;
+  const int64_t each = (tiles + kWaves - 1) / kWaves, most = kCus * groups_per_cu(p);
+  s.aligned = p.B * s.rows * each <= most;
+  s.each = static_cast<int>(each);
+  s.groups = static_cast<int>(s.aligned ? p.B * s.rows * each : most);
   return s;
 }
-// Splits a sequence can have at most, were it alone as long as the table.
-int64_t most_splits(const Shape& s) {
-  const int64_t tiles = (s.cap + kTileKeys - 1) / kTileKeys;
-  return std::min<int64_t>((tiles + kWaves - 1) / kWaves, kUnits);
-}
+// Whether a row may be cut.
+bool may_cut(const Shape& s) { return !s.aligned || s.cap > kWaves * kTileKeys; }
 
 void check_launch(const char* what) {
   const hipError_t e = hipGetLastError();
@@ -630,11 +751,9 @@ void check_launch(const char* what) {
 
 size_t paged_attention_scratch_bytes(const PagedParams& p, DType t) {
   const Shape s = shape_of(p);
-  if (p.B == 0 || most_splits(s) <= 1) return 0;
-  // A sequence of n > 1 splits has more than n / 2 of unit_tiles each, so the
-  // split sequences' rows have fewer than 2 kUnits of them in all.
-  const int64_t slots = std::min<int64_t>(2 * kUnits, p.B * s.rows * most_splits(s));
-  return static_cast<size_t>(slots) * s.heads * (p.D + 2) * sizeof(float);
+  if (p.B == 0 || !may_cut(s)) return 0;
+  return static_cast<size_t>(p.B) * s.rows * sizeof(Row) +
+         static_cast<size_t>(slot_of(s.groups, false)) * s.heads * (p.D + 2) * sizeof(float);
 }
 
 void launch_paged_attention(hipStream_t stream, const PagedParams& p, DType t, const void* q, const void* k_pages,
@@ -642,26 +761,22 @@ void launch_paged_attention(hipStream_t stream, const PagedParams& p, DType t, c
                             void* scratch) {
   if (p.B == 0) return;
   const Shape s = shape_of(p);
-  const int64_t rows = p.B * s.rows;
-  // Splits of unit_tiles tiles, and one that is short a row.
-  const int64_t units = std::min<int64_t>(rows * most_splits(s), rows + kUnits);
-  // The waves' outputs, [waves][heads][D].
-  const size_t lds = static_cast<size_t>(kWaves) * s.heads * p.D * sizeof(float);
   auto go = [&](auto tag) {
     using T = decltype(tag);
     const T *qp = static_cast<const T*>(q), *kp = static_cast<const T*>(k_pages), *vp = static_cast<const T*>(v_pages);
-    const dim3 grid(static_cast<uint32_t>(units)), block(kWaves * 64);
+    const dim3 grid(static_cast<uint32_t>(s.groups)), block(kWaves * 64);
     T* op = static_cast<T*>(out);
     float* sp = static_cast<float*>(scratch);
-#define PJRTX_PAGED(DIM)                                                                                      \
-  case DIM:                                                                                                   \
-    if (p.S % 16 == 0)                                                                                        \
-      hipLaunchKernelGGL((paged_tiles<T, DIM, true>), grid, block, lds, stream, s, qp, kp, vp, page_table,    \
-                         lengths, op, sp);                                                                    \
-    else                                                                                                      \
-      hipLaunchKernelGGL((paged_tiles<T, DIM, false>), grid, block, lds, stream, s, qp, kp, vp, page_table,   \
-                         lengths, op, sp);                                                                    \
+#define PJRTX_PAGED_AS(...) \
+  hipLaunchKernelGGL((__VA_ARGS__), grid, block, lds, stream, s, qp, kp, vp, page_table, lengths, op, sp)
+#define PJRTX_PAGED(DIM)                                                         \
+  case DIM:                                                                      \
+    if (p.S % 16 == 0 && s.aligned) PJRTX_PAGED_AS(paged_tiles<T, DIM, true, true>);   \
+    else if (p.S % 16 == 0) PJRTX_PAGED_AS(paged_tiles<T, DIM, true, false>);    \
+    else if (s.aligned) PJRTX_PAGED_AS(paged_tiles<T, DIM, false, true>);        \
+    else PJRTX_PAGED_AS(paged_tiles<T, DIM, false, false>);                      \
     break
+    size_t lds = static_cast<size_t>(kWaves) * s.heads * p.D * sizeof(float);  // the waves' outputs
     switch (p.D) {
       PJRTX_PAGED(32);
       PJRTX_PAGED(64);
@@ -670,12 +785,16 @@ void launch_paged_attention(hipStream_t stream, const PagedParams& p, DType t, c
       PJRTX_PAGED(192);
       PJRTX_PAGED(256);
       default:
-        hipLaunchKernelGGL((paged_any<T>), grid, block, 0, stream, s, qp, kp, vp, page_table, lengths, op, sp);
+        lds = 0;
+        if (s.aligned) PJRTX_PAGED_AS(paged_any<T, true>);
+        else PJRTX_PAGED_AS(paged_any<T, false>);
     }
+#undef PJRTX_PAGED_AS
 #undef PJRTX_PAGED
-    if (scratch)
-      hipLaunchKernelGGL((paged_combine<T>), dim3(static_cast<uint32_t>(p.B * p.Hq)), dim3(256), 0, stream, s, lengths,
-                         sp, op);
+    if (!sp) return;
+    const dim3 heads(static_cast<uint32_t>(p.B * p.Hq));
+    if (p.D % 4 == 0) hipLaunchKernelGGL((paged_combine<T, 4>), heads, block, 0, stream, s, sp, op);
+    else hipLaunchKernelGGL((paged_combine<T, 1>), heads, block, 0, stream, s, sp, op);
   };
   if (t == DType::kF32) go(float());
   else if (t == DType::kBF16) go(bf16_t());

@@ -106,9 +106,13 @@ void lower_paged_attention(const Checker& c, Op* op) {
   const int64_t window = c.integer("window", 0);
   c.need(window >= 0, "window must not be negative");
   c.within(q.dims[2] <= 512, "head dim above 512");
-  c.within(table.dims[1] * k.dims[2] <= kMaxIndex, "a page table of more than 2^31 - 1 keys");
-  c.within(q.dims[0] * q.dims[1] + 512 <= kMaxGroups, "too many query heads");
-  c.within(q.dims[0] * ((table.dims[1] * k.dims[2] + 31) / 32) <= kMaxIndex, "too many keys in the page table");
+  // keys are counted in 32 bits, up to a tile past the last
+  c.within(table.dims[1] <= kMaxIndex && table.dims[1] * k.dims[2] <= kMaxIndex - 64,
+           "a page table of more than 2^31 - 65 keys");
+  c.within(q.dims[0] <= kMaxGroups && q.dims[1] <= kMaxGroups && q.dims[0] * q.dims[1] <= kMaxGroups, "too many query heads");
+  // tiles of 32 keys of every head are counted in 32 bits
+  c.within(q.dims[0] * q.dims[1] * ((table.dims[1] * k.dims[2] + 31) / 32 + 1) <= kMaxIndex,
+           "too many keys in the page table");
   op->kind = OpKind::kPagedAttention;
   op->oper.scale = scale;
   op->oper.window = window;
