@@ -2,10 +2,12 @@
 // likeliest tokens, in one pass over the logits; and their gradient.
 //
 // A row is split over workgroups, which read it in chunks of 8192 elements
-// held in registers. Each thread keeps an online softmax of its own (largest
-// x so far m, l = sum e^(x-m), a = sum e^(x-m) (x-m)), from which lse = m +
-// log l and entropy = log l - a / l: the entropy's terms are taken about m,
-// not about zero, so nothing large cancels. Elements that may be among the
+// held in registers. Each thread keeps an online softmax of its own, in powers
+// of two: m = x log2(e) of the largest x so far, l = sum 2^y and a = sum 2^y y
+// with y = x log2(e) - m, from which lse = (m + log2 l) ln 2 and entropy =
+// (log2 l - a / l) ln 2. The entropy's terms are taken about m, not about zero,
+// so nothing large cancels, and m is the number that is subtracted, so its own
+// rounding is in no result. Elements that may be among the
 // row's top_k (bounded below by the threads' maxima, then by the top_k found so
 // far) go to a list in LDS and are ranked there by value, then by lowest index.
 // logprobs_join folds a row's splits.
@@ -42,17 +44,27 @@ __device__ __forceinline__ uint64_t key_of(float x, int64_t i) {
   return ((uint64_t)order_of(x) << 32) | (uint32_t)~(uint32_t)i;
 }
 
+constexpr float kLn2 = 0.69314718055994530942f;
+
 // One thread's or split's softmax state.
 struct Soft {
   float m, l, a;
 };
-__device__ __forceinline__ Soft join(const Soft& x, const Soft& y) {
+// The state about the larger maximum m >= s.m.
+__device__ __forceinline__ void raise(Soft& s, float m) {
+  // A side of no elements has l = a = 0 at -inf: its shift is made finite.
+  const float d = fmaxf(s.m - m, -1e4f), f = exp2f(d);
+  s.a = f * (s.a + d * s.l);
+  s.l *= f;
+  s.m = m;
+}
+__device__ __forceinline__ Soft join(Soft x, Soft y) {
   const float m = fmaxf(x.m, y.m);
-  if (m == -INFINITY) return {m, x.l + y.l, x.a + y.a};  // 0s, or NaNs
-  // A side of no elements has l = a = 0 at m = -inf: its shift is finite here.
-  const float dx = fmaxf(x.m - m, -1e4f), dy = fmaxf(y.m - m, -1e4f);
-  const float fx = exp2f(dx * kLog2e), fy = exp2f(dy * kLog2e);
-  return {m, x.l * fx + y.l * fy, fx * (x.a + dx * x.l) + fy * (y.a + dy * y.l)};
+  if (m != -INFINITY) {  // else 0s, or NaNs
+    raise(x, m);
+    raise(y, m);
+  }
+  return {m, x.l + y.l, x.a + y.a};
 }
 
 // The split's results: {m, l, a}, then top_k keys, largest first, 0 past the last.
@@ -100,7 +112,7 @@ __device__ __forceinline__ int64_t read_token(const void* tokens, int bytes, int
 }
 
 // A workgroup's share of a row: elements [lo, hi).
-template <typename T, bool kTop>
+template <typename T, bool kTop, bool kStream>
 __global__ void __launch_bounds__(kThreads)
     logprobs_split(LogprobsParams p, int nsplit, int64_t per, const T* __restrict__ logits,
                    uint32_t* __restrict__ part) {
@@ -125,7 +137,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int64_t at = base + (int64_t)(i * kThreads + tid) * E;
-      v[i] = load_vec<T>(x + std::min(at, p.V - 1), hi - at, (T)-INFINITY);
+      v[i] = load_vec<T, kStream>(x + std::min(at, p.V - 1), hi - at, (T)-INFINITY);
     }
     float cm = -INFINITY;  // NaN where one is
 #pragma unroll
@@ -141,23 +153,18 @@ __global__ void __launch_bounds__(kThreads)
       }
       if (tid == 0) count_s = 0;
     }
-    const float m = fmaxf(s.m, cm);
-    if (m > s.m) {  // also the first finite chunk, from l = a = 0
-      const float d = fmaxf(s.m - m, -1e4f), f = exp2f(d * kLog2e);
-      s.a = f * (s.a + d * s.l);
-      s.l *= f;
-      s.m = m;
-    }
+    const float m = fmaxf(s.m, cm * kLog2e);
+    if (m > s.m) raise(s, m);  // also the first finite chunk, from l = a = 0
     const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         // -inf weighs nothing: its distance is made finite for a's product.
-        const float d = __builtin_elementwise_maximum((float)v[i][e] - ref, -1e4f);
-        const float w = __builtin_amdgcn_exp2f(d * kLog2e);
+        const float y = __builtin_elementwise_maximum(fmaf((float)v[i][e], kLog2e, -ref), -1e4f);
+        const float w = __builtin_amdgcn_exp2f(y);
         s.l += w;
-        s.a = fmaf(w, d, s.a);
+        s.a = fmaf(w, y, s.a);
       }
     if constexpr (kTop) {
       const int64_t left = hi - base;
@@ -169,15 +176,19 @@ __global__ void __launch_bounds__(kThreads)
                                : value_of(std::min(std::min(kth[0], kth[1]), std::min(kth[2], kth[3])));
       auto may = [&](float y) { return full ? !(y <= bound) : !(y < bound); };
       if (may(cm)) {
+        // Which of the thread's elements, in bits; the few are read again.
+        uint32_t bits = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (may((float)v[i][e])) {
-              const int64_t index = (int64_t)(i * kThreads + tid) * E + e;
-              const int at = index < left ? atomicAdd(&count_s, 1) : kCandidates;
-              if (at < kCandidates) cand[at] = key_of((float)v[i][e], base + index);
-            }
+          for (int e = 0; e < E; ++e) bits |= may((float)v[i][e]) ? 1u << (i * E + e) : 0u;
+        while (bits) {
+          const int j = __ffs(bits) - 1;
+          bits &= bits - 1;
+          const int64_t index = (int64_t)(j / E * kThreads + tid) * E + j % E;
+          const int at = index < left ? atomicAdd(&count_s, 1) : kCandidates;
+          if (at < kCandidates) cand[at] = key_of((float)x[base + index], base + index);
+        }
       }
       __syncthreads();
       int n = count_s;
@@ -259,27 +270,29 @@ __global__ void __launch_bounds__(64)
   }
   for (int d = 1; d < nsplit; d <<= 1)
     s = join(s, Soft{__shfl_xor(s.m, d), __shfl_xor(s.l, d), __shfl_xor(s.a, d)});
-  const float log_l = logf(s.l);
-  const float lse = __shfl(s.m + log_l, 0);
+  const float log_l = log2f(s.l);
+  const float lse = __shfl(fmaf(s.m, kLn2, log_l * kLn2), 0);
   if (lane == 0) {
     logprobs[row] = known ? chosen - lse : 0.f;
-    entropy[row] = log_l - s.a / s.l;
+    entropy[row] = (log_l - s.a / s.l) * kLn2;
     lse_out[row] = lse;
   }
   if (p.top_k == 0) return;
   __syncthreads();
-  int next = 0;
-  uint64_t mine = lane < nsplit ? keys[lane * p.top_k] : 0;
+  int next = 0;  // the lane's next key
+  auto key_at = [&](int i) { return lane < nsplit && i < p.top_k ? keys[lane * p.top_k + i] : 0; };
+  uint64_t mine = key_at(0);
   uint64_t found[kLogprobsMaxTopK / 64] = {};  // lane i: the keys of ranks i, i + 64, ...
   for (int k = 0; k < p.top_k; ++k) {
     const uint32_t high = wave_max_u((uint32_t)(mine >> 32));
-    const bool tied = (uint32_t)(mine >> 32) == high && mine != 0;
-    const uint32_t low = wave_max_u(tied ? (uint32_t)mine : 0u);
+    const bool has = (uint32_t)(mine >> 32) == high && mine != 0;
+    const uint64_t who = __ballot(has);
+    // Of equal values the lowest index, which is the largest complement.
+    const uint32_t low = __popcll(who) == 1
+                             ? (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)mine, __ffsll((unsigned long long)who) - 1)
+                             : wave_max_u(has ? (uint32_t)mine : 0u);
     const uint64_t key = (uint64_t)high << 32 | low;
-    if (mine == key) {
-      ++next;
-      mine = next < p.top_k ? keys[lane * p.top_k + next] : 0;
-    }
+    if (mine == key) mine = key_at(++next);
 #pragma unroll
     for (int j = 0; j < kLogprobsMaxTopK / 64; ++j)
       if (k == j * 64 + lane) found[j] = key;
@@ -294,7 +307,7 @@ __global__ void __launch_bounds__(64)
 }
 
 // Elementwise over the logits, a row's numbers read once a workgroup.
-template <typename T>
+template <typename T, bool kStream>
 __global__ void __launch_bounds__(kThreads)
     logprobs_grad(LogprobsParams p, int nsplit, const T* __restrict__ logits, const void* __restrict__ tokens,
                   const float* __restrict__ lse, const float* __restrict__ entropy,
@@ -308,7 +321,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int64_t at = base + (int64_t)(i * kThreads + threadIdx.x) * E;
-    v[i] = load_vec<T>(x + std::min(at, p.V - 1), p.V - at, (T)0.f);
+    v[i] = load_vec<T, kStream>(x + std::min(at, p.V - 1), p.V - at, (T)0.f);
   }
   const int64_t token = read_token(tokens, p.token_bytes, row);
   const bool known = token >= 0 && token < p.V;
@@ -330,7 +343,7 @@ __global__ void __launch_bounds__(kThreads)
       if (at + e == token) y += g;
       o[e] = (T)y;
     }
-    store_vec<T>(dx + row * p.V + at, n, o);
+    store_vec<T, kStream>(dx + row * p.V + at, n, o);
   }
 }
 
@@ -370,8 +383,14 @@ void launch_token_logprobs(hipStream_t s, const LogprobsParams& p, DType t, cons
   auto go = [&](auto tag) {
     using T = decltype(tag);
     const T* x = static_cast<const T*>(logits);
-    if (p.top_k) hipLaunchKernelGGL((logprobs_split<T, true>), grid, block, 0, s, p, sp.n, sp.per, x, part);
-    else hipLaunchKernelGGL((logprobs_split<T, false>), grid, block, 0, s, p, sp.n, sp.per, x, part);
+    const bool stream = p.rows * p.V * static_cast<int64_t>(sizeof(T)) >= kStreamBytes;
+#define PJRTX_LOGPROBS(TOP, STREAM) \
+  hipLaunchKernelGGL((logprobs_split<T, TOP, STREAM>), grid, block, 0, s, p, sp.n, sp.per, x, part)
+    if (p.top_k && stream) PJRTX_LOGPROBS(true, true);
+    else if (p.top_k) PJRTX_LOGPROBS(true, false);
+    else if (stream) PJRTX_LOGPROBS(false, true);
+    else PJRTX_LOGPROBS(false, false);
+#undef PJRTX_LOGPROBS
     hipLaunchKernelGGL((logprobs_join<T>), dim3(static_cast<uint32_t>(p.rows)), dim3(64), 0, s, p, sp.n, x, tokens, part, logprobs, entropy, lse,
                        top_logprobs, top_tokens);
   };
@@ -388,9 +407,15 @@ void launch_token_logprobs_grad(hipStream_t s, const LogprobsParams& p, DType t,
   const int n = static_cast<int>((p.V + kChunk - 1) / kChunk);
   auto go = [&](auto tag) {
     using T = decltype(tag);
-    hipLaunchKernelGGL((logprobs_grad<T>), dim3(static_cast<uint32_t>(p.rows * n)), dim3(kThreads), 0, s, p, n,
-                       static_cast<const T*>(logits), tokens, lse, entropy, d_logprobs, d_entropy,
-                       static_cast<T*>(d_logits));
+    const dim3 grid(static_cast<uint32_t>(p.rows * n)), block(kThreads);
+    const T* x = static_cast<const T*>(logits);
+    T* dx = static_cast<T*>(d_logits);
+    if (p.rows * p.V * static_cast<int64_t>(sizeof(T)) >= kStreamBytes)
+      hipLaunchKernelGGL((logprobs_grad<T, true>), grid, block, 0, s, p, n, x, tokens, lse, entropy, d_logprobs,
+                         d_entropy, dx);
+    else
+      hipLaunchKernelGGL((logprobs_grad<T, false>), grid, block, 0, s, p, n, x, tokens, lse, entropy, d_logprobs,
+                         d_entropy, dx);
   };
   if (t == DType::kF32) go(float());
   else if (t == DType::kBF16) go(bf16_t());

@@ -22,21 +22,31 @@ struct Vec {
   typedef type unaligned __attribute__((aligned(sizeof(T))));
 };
 
+// Tensors of at least this size are read and written past the caches' lines
+// that others use (kStream below): they do not stay in an L2 anyway.
+constexpr int64_t kStreamBytes = int64_t(32) << 20;
+
 // Elements [0, n) of the vector at p, the others `fill`. n >= kVecElems is the
 // common case: one load.
-template <typename T>
+template <typename T, bool kStream = false>
 __device__ __forceinline__ typename Vec<T>::type load_vec(const T* p, int64_t n, T fill) {
-  if (n >= kVecElems<T>) return *reinterpret_cast<const typename Vec<T>::unaligned*>(p);
+  if (n >= kVecElems<T>) {
+    const auto* at = reinterpret_cast<const typename Vec<T>::unaligned*>(p);
+    if constexpr (kStream) return __builtin_nontemporal_load(at);
+    else return *at;
+  }
   typename Vec<T>::type v;
 #pragma unroll
   for (int e = 0; e < kVecElems<T>; ++e) v[e] = e < n ? p[e] : fill;
   return v;
 }
 
-template <typename T>
+template <typename T, bool kStream = false>
 __device__ __forceinline__ void store_vec(T* p, int64_t n, const typename Vec<T>::type& v) {
   if (n >= kVecElems<T>) {
-    *reinterpret_cast<typename Vec<T>::unaligned*>(p) = v;
+    auto* at = reinterpret_cast<typename Vec<T>::unaligned*>(p);
+    if constexpr (kStream) __builtin_nontemporal_store(v, at);
+    else *at = v;
     return;
   }
 #pragma unroll

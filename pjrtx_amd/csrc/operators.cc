@@ -128,6 +128,10 @@ void lower_paged_append(const Checker& c, Op* op) {
   c.need(slots.rank() == 1 && is_index(slots.dtype) && slots.dims[0] == kn.dims[0], "slots must be s32 or s64 [rows]");
   c.need(c.out(0) == k && c.out(1) == k, "the results must have the pages' shape and type");
   c.within(kn.dims[0] <= kMaxGroups, "too many rows");
+  c.within(kn.dims[1] <= (int64_t(1) << 24) && kn.dims[2] <= (int64_t(1) << 24) &&
+               kn.dims[1] * kn.dims[2] <= (int64_t(1) << 24),
+           "rows of more than 2^24 elements");
+  c.within(k.dims[0] * k.dims[2] <= kMaxIndex, "more than 2^31 - 1 slots");
   op->kind = OpKind::kPagedAppend;
 }
 
