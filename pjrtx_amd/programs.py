@@ -127,3 +127,29 @@ def topk_logits(rows: int = 64, vocab: int = 128256, k: int = 50) -> str:
     logits = b.param((rows, vocab), "bf16")
     v, i = b.top_k(logits, k)
     return b.build([v, i])
+
+
+def lm_head_loss(rows: int, d_model: int, vocab: int, entropy_weight: float = 0.0, eps: float = 1e-5) -> str:
+    """The end of a decoder's training step and its gradients: h, t =
+    add_rms_norm(x, residual, gain); logits = h.W; loss = the mean over rows
+    whose target is in the vocabulary of -log p(target), less entropy_weight of
+    the entropy. Returns (loss, d x = d residual, d gain, d W), everything but
+    the loss bf16."""
+    b = Builder("jit_lm_head_loss")
+    x, residual = b.param((rows, d_model), "bf16"), b.param((rows, d_model), "bf16")
+    gain, w, targets = b.param((d_model,), "bf16"), b.param((d_model, vocab), "bf16"), b.param((rows,), "s32")
+    h, t = b.add_rms_norm(x, residual, gain, eps)
+    logits = b.dot_general(h, w, contract=((1,), (0,)))
+    lp, entropy, lse = b.token_logprobs(logits, targets)
+    live = b.convert(b.and_(b.compare("GE", targets, b.scalar_like(0, targets)),
+                            b.compare("LT", targets, b.scalar_like(vocab, targets))), "f32")
+    share = b.divide(live, b.broadcast_in_dim(b.sum(live, [0]), live.shape, []))
+    gained = b.add(lp, b.multiply(entropy, b.scalar_like(entropy_weight, entropy)))
+    loss = b.negate(b.sum(b.multiply(share, gained), [0]))
+    d_lp = b.negate(share)
+    d_logits = b.token_logprobs_grad(logits, targets, lse, entropy, d_lp,
+                                     b.multiply(d_lp, b.scalar_like(entropy_weight, d_lp)))
+    d_h = b.dot_general(d_logits, w, contract=((1,), (1,)))
+    d_w = b.dot_general(h, d_logits, contract=((0,), (0,)))
+    d_x, d_gain = b.add_rms_norm_grad(d_h, None, t, gain, eps)
+    return b.build([loss, d_x, d_gain, d_w])
