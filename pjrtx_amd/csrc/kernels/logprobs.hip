@@ -111,11 +111,32 @@ __device__ __forceinline__ int64_t read_token(const void* tokens, int bytes, int
   return bytes == 8 ? static_cast<const int64_t*>(tokens)[i] : (int64_t)static_cast<const int32_t*>(tokens)[i];
 }
 
-// A workgroup's share of a row: elements [lo, hi).
+struct Results {
+  float *logprobs, *entropy, *lse, *top_logprobs;
+  int32_t* top_tokens;
+};
+__device__ __forceinline__ float lse_of(const Soft& s) { return fmaf(s.m, kLn2, log2f(s.l) * kLn2); }
+// By one thread: the row's numbers, `chosen` its token's logit.
+__device__ __forceinline__ void write_row(const Results& r, int64_t row, const Soft& s, bool known, float chosen) {
+  const float lse = lse_of(s);
+  r.logprobs[row] = known ? chosen - lse : 0.f;
+  r.entropy[row] = (log2f(s.l) - s.a / s.l) * kLn2;
+  r.lse[row] = lse;
+}
+// By the workgroup: the row's likeliest tokens, ranked.
+__device__ __forceinline__ void write_top(const Results& r, int64_t row, float lse, const uint64_t* best, int top_k) {
+  for (int i = threadIdx.x; i < top_k; i += kThreads) {
+    r.top_logprobs[row * top_k + i] = value_of((uint32_t)(best[i] >> 32)) - lse;
+    r.top_tokens[row * top_k + i] = (int32_t)~(uint32_t)best[i];
+  }
+}
+
+// A workgroup's share of a row: elements [lo, hi). A row of one share is
+// finished here.
 template <typename T, bool kTop, bool kStream>
 __global__ void __launch_bounds__(kThreads)
     logprobs_split(LogprobsParams p, int nsplit, int64_t per, const T* __restrict__ logits,
-                   uint32_t* __restrict__ part) {
+                   const void* __restrict__ tokens, uint32_t* __restrict__ part, Results r) {
   constexpr int E = kVecElems<T>;
   constexpr int NV = kChunk / kThreads / E;
   constexpr int kWaves = kThreads / 64;
@@ -170,24 +191,30 @@ __global__ void __launch_bounds__(kThreads)
       const int64_t left = hi - base;
       __syncthreads();
       // Elements at the bound count in the first chunk; behind top_k keys that
-      // were found before (at lower indices) they do not. NaNs always do.
-      const bool full = held == p.top_k;
-      const float bound = full ? value_of((uint32_t)(best[turn][p.top_k - 1] >> 32))
-                               : value_of(std::min(std::min(kth[0], kth[1]), std::min(kth[2], kth[3])));
-      auto may = [&](float y) { return full ? !(y <= bound) : !(y < bound); };
+      // were found before (at lower indices) the next float is the bound. NaNs
+      // always count.
+      const float bound = value_of(held == p.top_k ? (uint32_t)(best[turn][p.top_k - 1] >> 32) + 1
+                                                   : std::min(std::min(kth[0], kth[1]), std::min(kth[2], kth[3])));
+      auto may = [&](float y) { return !(y < bound); };
       if (may(cm)) {
-        // Which of the thread's elements, in bits; the few are read again.
+        // Which of the thread's elements, in bits, and the last one's value:
+        // most threads have one. Others are read again.
         uint32_t bits = 0;
+        float value = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-          for (int e = 0; e < E; ++e) bits |= may((float)v[i][e]) ? 1u << (i * E + e) : 0u;
-        while (bits) {
-          const int j = __ffs(bits) - 1;
-          bits &= bits - 1;
+          for (int e = 0; e < E; ++e) {
+            const bool yes = may((float)v[i][e]);
+            bits |= yes ? 1u << (i * E + e) : 0u;
+            value = yes ? (float)v[i][e] : value;
+          }
+        for (bool read = false; bits; read = true) {
+          const int j = 31 - __clz(bits);
+          bits ^= 1u << j;
           const int64_t index = (int64_t)(j / E * kThreads + tid) * E + j % E;
           const int at = index < left ? atomicAdd(&count_s, 1) : kCandidates;
-          if (at < kCandidates) cand[at] = key_of((float)x[base + index], base + index);
+          if (at < kCandidates) cand[at] = key_of(read ? (float)x[base + index] : value, base + index);
         }
       }
       __syncthreads();
@@ -228,9 +255,18 @@ __global__ void __launch_bounds__(kThreads)
   for (int d = 32; d >= 1; d >>= 1) s = join(s, Soft{__shfl_xor(s.m, d), __shfl_xor(s.l, d), __shfl_xor(s.a, d)});
   if ((tid & 63) == 0) soft_s[tid >> 6] = s;
   __syncthreads();
+  const Soft t = join(join(soft_s[0], soft_s[1]), join(soft_s[2], soft_s[3]));
+  if (nsplit == 1) {
+    if (tid == 0) {
+      const int64_t token = read_token(tokens, p.token_bytes, row);
+      const bool known = token >= 0 && token < p.V;
+      write_row(r, row, t, known, known ? (float)x[token] : 0.f);
+    }
+    if constexpr (kTop) write_top(r, row, lse_of(t), best[turn], p.top_k);
+    return;
+  }
   uint32_t* out = part + (row * nsplit + split) * split_words(p.top_k);
   if (tid == 0) {
-    const Soft t = join(join(soft_s[0], soft_s[1]), join(soft_s[2], soft_s[3]));
     out[0] = __builtin_bit_cast(uint32_t, t.m);
     out[1] = __builtin_bit_cast(uint32_t, t.l);
     out[2] = __builtin_bit_cast(uint32_t, t.a);
@@ -244,66 +280,58 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// One wave a row, a lane a split: the softmax states folded by halves, and the
-// splits' ordered keys merged, the largest of the lanes' next ones at a time.
+// The splits of a row: their softmax states folded by halves (a lane each), and
+// their keys ranked. Of nsplit ordered lists the ceil(top_k / nsplit)-th keys
+// bound the top_k from below: few keys are at or above the least of them.
 template <typename T>
-__global__ void __launch_bounds__(64)
+__global__ void __launch_bounds__(kThreads)
     logprobs_join(LogprobsParams p, int nsplit, const T* __restrict__ logits, const void* __restrict__ tokens,
-                  const uint32_t* __restrict__ part, float* __restrict__ logprobs, float* __restrict__ entropy,
-                  float* __restrict__ lse_out, float* __restrict__ top_logprobs, int32_t* __restrict__ top_tokens) {
+                  const uint32_t* __restrict__ part, Results r) {
   __shared__ uint64_t keys[kJoinKeys];
+  __shared__ uint64_t best[kLogprobsMaxTopK];
+  __shared__ int count_s;
   const int64_t row = blockIdx.x;
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x & 63;
   const int64_t words = split_words(p.top_k);
   const uint32_t* in = part + row * nsplit * words;
-  const int64_t token = read_token(tokens, p.token_bytes, row);
-  const bool known = token >= 0 && token < p.V;
-  const float chosen = known ? (float)logits[row * p.V + token] : 0.f;
-  for (int i = lane; i < nsplit * p.top_k; i += 64) {
-    const uint32_t* w = in + (i / p.top_k) * words + 4 + 2 * (i % p.top_k);
-    keys[i] = (uint64_t)w[1] << 32 | w[0];
-  }
+  // Each wave folds the states, and takes the bound, alone.
   Soft s = {-INFINITY, 0.f, 0.f};
+  uint32_t high = ~0u;
   if (lane < nsplit) {
     const uint32_t* w = in + lane * words;
     s = {__builtin_bit_cast(float, w[0]), __builtin_bit_cast(float, w[1]), __builtin_bit_cast(float, w[2])};
+    if (p.top_k) high = w[4 + 2 * ((p.top_k + nsplit - 1) / nsplit - 1) + 1];
   }
+  const int n = nsplit * p.top_k;
+  constexpr int kMine = kJoinKeys / kThreads;
+  uint64_t mine[kMine];
+#pragma unroll
+  for (int j = 0; j < kMine; ++j) {
+    const int i = j * kThreads + threadIdx.x;
+    mine[j] = 0;
+    if (i < n) {
+      const int split = i / p.top_k;
+      const uint32_t* w = in + split * words + 4 + 2 * (i - split * p.top_k);
+      mine[j] = (uint64_t)w[1] << 32 | w[0];
+    }
+  }
+  const int64_t token = read_token(tokens, p.token_bytes, row);
+  const bool known = token >= 0 && token < p.V;
+  const float chosen = known ? (float)logits[row * p.V + token] : 0.f;
+  if (threadIdx.x == 0) count_s = 0;
   for (int d = 1; d < nsplit; d <<= 1)
     s = join(s, Soft{__shfl_xor(s.m, d), __shfl_xor(s.l, d), __shfl_xor(s.a, d)});
-  const float log_l = log2f(s.l);
-  const float lse = __shfl(fmaf(s.m, kLn2, log_l * kLn2), 0);
-  if (lane == 0) {
-    logprobs[row] = known ? chosen - lse : 0.f;
-    entropy[row] = (log_l - s.a / s.l) * kLn2;
-    lse_out[row] = lse;
-  }
+  if (threadIdx.x == 0) write_row(r, row, s, known, chosen);
   if (p.top_k == 0) return;
+  const uint32_t bound = ~wave_max_u(~high);
   __syncthreads();
-  int next = 0;  // the lane's next key
-  auto key_at = [&](int i) { return lane < nsplit && i < p.top_k ? keys[lane * p.top_k + i] : 0; };
-  uint64_t mine = key_at(0);
-  uint64_t found[kLogprobsMaxTopK / 64] = {};  // lane i: the keys of ranks i, i + 64, ...
-  for (int k = 0; k < p.top_k; ++k) {
-    const uint32_t high = wave_max_u((uint32_t)(mine >> 32));
-    const bool has = (uint32_t)(mine >> 32) == high && mine != 0;
-    const uint64_t who = __ballot(has);
-    // Of equal values the lowest index, which is the largest complement.
-    const uint32_t low = __popcll(who) == 1
-                             ? (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)mine, __ffsll((unsigned long long)who) - 1)
-                             : wave_max_u(has ? (uint32_t)mine : 0u);
-    const uint64_t key = (uint64_t)high << 32 | low;
-    if (mine == key) mine = key_at(++next);
 #pragma unroll
-    for (int j = 0; j < kLogprobsMaxTopK / 64; ++j)
-      if (k == j * 64 + lane) found[j] = key;
-  }
-#pragma unroll
-  for (int j = 0; j < kLogprobsMaxTopK / 64; ++j) {
-    const int i = j * 64 + lane;
-    if (i >= p.top_k) continue;
-    top_logprobs[row * p.top_k + i] = value_of((uint32_t)(found[j] >> 32)) - lse;
-    top_tokens[row * p.top_k + i] = (int32_t)~(uint32_t)found[j];
-  }
+  for (int j = 0; j < kMine; ++j)
+    if (mine[j] != 0 && (uint32_t)(mine[j] >> 32) >= bound) keys[atomicAdd(&count_s, 1)] = mine[j];
+  __syncthreads();
+  rank_keys(keys, count_s, best, 0, best, p.top_k);
+  __syncthreads();
+  write_top(r, row, __shfl(lse_of(s), 0), best, p.top_k);
 }
 
 // Elementwise over the logits, a row's numbers read once a workgroup.
@@ -347,19 +375,29 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// Splits of a row: enough workgroups for the chip, whole chunks each, and no
-// more keys than the join ranks.
+// Splits of a row, whole chunks each: those of the least estimated time, in
+// chunks, of the rounds of workgroups (4 a CU at once) and of the join (64 x
+// 128256 bf16: 1 / 8 / 16 splits a row take ...).
 struct Split {
   int n;
   int64_t per;
 };
 Split split_of(const LogprobsParams& p) {
+  constexpr int64_t kAtOnce = 1024;
+  constexpr double kJoin = 0.7;
   const int64_t chunks = (p.V + kChunk - 1) / kChunk;
-  int64_t want = std::max<int64_t>(1, (1024 + p.rows - 1) / std::max<int64_t>(1, p.rows));
-  want = std::min<int64_t>(want, p.top_k ? std::min(kJoinSplits, kJoinKeys / p.top_k) : kJoinSplits);
-  const int64_t n = std::max<int64_t>(1, std::min(chunks, want));
-  const int64_t per = (chunks + n - 1) / n * kChunk;
-  return {static_cast<int>((p.V + per - 1) / per), per};
+  const int64_t most = std::min<int64_t>(chunks, p.top_k ? std::min(kJoinSplits, kJoinKeys / p.top_k) : kJoinSplits);
+  int64_t best = chunks;
+  double least = INFINITY;
+  for (int64_t n = 1; n <= most; ++n) {
+    const int64_t per = (chunks + n - 1) / n;
+    const double time = static_cast<double>((p.rows * n + kAtOnce - 1) / kAtOnce * per) + (n > 1 ? kJoin : 0);
+    if (time < least) {
+      least = time;
+      best = per;
+    }
+  }
+  return {static_cast<int>((chunks + best - 1) / best), best * kChunk};
 }
 
 void check_launch(const char* what) {
@@ -370,7 +408,8 @@ void check_launch(const char* what) {
 }  // namespace
 
 size_t token_logprobs_scratch_bytes(const LogprobsParams& p, DType t) {
-  return static_cast<size_t>(p.rows) * split_of(p).n * split_words(p.top_k) * sizeof(uint32_t);
+  const int n = split_of(p).n;
+  return n > 1 ? static_cast<size_t>(p.rows) * n * split_words(p.top_k) * sizeof(uint32_t) : 0;
 }
 
 void launch_token_logprobs(hipStream_t s, const LogprobsParams& p, DType t, const void* logits, const void* tokens,
@@ -380,19 +419,21 @@ void launch_token_logprobs(hipStream_t s, const LogprobsParams& p, DType t, cons
   const Split sp = split_of(p);
   const dim3 grid(static_cast<uint32_t>(p.rows * sp.n)), block(kThreads);
   uint32_t* part = static_cast<uint32_t*>(scratch);
+  const Results r = {logprobs, entropy, lse, top_logprobs, top_tokens};
   auto go = [&](auto tag) {
     using T = decltype(tag);
     const T* x = static_cast<const T*>(logits);
     const bool stream = p.rows * p.V * static_cast<int64_t>(sizeof(T)) >= kStreamBytes;
 #define PJRTX_LOGPROBS(TOP, STREAM) \
-  hipLaunchKernelGGL((logprobs_split<T, TOP, STREAM>), grid, block, 0, s, p, sp.n, sp.per, x, part)
+  hipLaunchKernelGGL((logprobs_split<T, TOP, STREAM>), grid, block, 0, s, p, sp.n, sp.per, x, tokens, part, r)
     if (p.top_k && stream) PJRTX_LOGPROBS(true, true);
     else if (p.top_k) PJRTX_LOGPROBS(true, false);
     else if (stream) PJRTX_LOGPROBS(false, true);
     else PJRTX_LOGPROBS(false, false);
 #undef PJRTX_LOGPROBS
-    hipLaunchKernelGGL((logprobs_join<T>), dim3(static_cast<uint32_t>(p.rows)), dim3(64), 0, s, p, sp.n, x, tokens, part, logprobs, entropy, lse,
-                       top_logprobs, top_tokens);
+    if (sp.n > 1)
+      hipLaunchKernelGGL((logprobs_join<T>), dim3(static_cast<uint32_t>(p.rows)), block, 0, s, p, sp.n, x, tokens, part,
+                         r);
   };
   if (t == DType::kF32) go(float());
   else if (t == DType::kBF16) go(bf16_t());
