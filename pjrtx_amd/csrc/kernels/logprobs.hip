@@ -375,23 +375,26 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// Splits of a row, whole chunks each: those of the least estimated time, in
-// chunks, of the rounds of workgroups (4 a CU at once) and of the join (64 x
-// 128256 bf16: 1 / 8 / 16 splits a row take ...).
+// Splits of a row, whole chunks each: those of the least estimated time, in the
+// 5 us that 4 workgroups on each CU take for a chunk. Many workgroups: a chunk
+// each costs 0.45 more to begin and end, and the last round is half empty. Few:
+// the time of one alone, 1.8 and 0.25 a chunk. The join: 0.45 and 0.05 a split.
+// (bf16, 20 likeliest, 64 x 128256: 16 splits a row 10.8 + 6.9 us, 8 splits 11.7
+// + 5.1; 600 x 128256, 5 likeliest: 16 splits 65 + 5 us, 1 split 53.)
 struct Split {
   int n;
   int64_t per;
 };
 Split split_of(const LogprobsParams& p) {
-  constexpr int64_t kAtOnce = 1024;
-  constexpr double kJoin = 0.7;
   const int64_t chunks = (p.V + kChunk - 1) / kChunk;
   const int64_t most = std::min<int64_t>(chunks, p.top_k ? std::min(kJoinSplits, kJoinKeys / p.top_k) : kJoinSplits);
   int64_t best = chunks;
   double least = INFINITY;
   for (int64_t n = 1; n <= most; ++n) {
     const int64_t per = (chunks + n - 1) / n;
-    const double time = static_cast<double>((p.rows * n + kAtOnce - 1) / kAtOnce * per) + (n > 1 ? kJoin : 0);
+    const double rounds = static_cast<double>(p.rows) * n / 1024, group = per + 0.45;
+    const double time = std::max(rounds * group + (rounds > 1 ? 0.5 * group : 0), 1.8 + 0.25 * per) +
+                        (n > 1 ? 0.45 + 0.05 * n : 0);
     if (time < least) {
       least = time;
       best = per;
