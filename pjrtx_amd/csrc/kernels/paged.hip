@@ -135,7 +135,8 @@ __device__ __forceinline__ int row_of(const Shape& s, const int32_t* table, int6
 }
 
 // What the workgroup that starts a row leaves for paged_combine, before the
-// slots: the row's parts are that workgroup's and the n - 1 after it.
+// slots (unless rows start on a workgroup's first tile): the row's parts are
+// that workgroup's and the n - 1 after it.
 struct Row {
   uint32_t group, n;
 };
@@ -177,7 +178,6 @@ __device__ __forceinline__ void set_unit(const Shape& s, Unit* u, uint32_t r, co
 template <bool kAligned, typename F>
 __device__ __forceinline__ void for_parts(const Shape& s, const int32_t* lengths, float* scratch, const F& part) {
   Unit u;
-  Row* rows = reinterpret_cast<Row*>(scratch);
   if constexpr (kAligned) {
     // Row by row, as many workgroups each as the table's keys could take.
     const uint32_t row = blockIdx.x / (uint32_t)s.each, tile = (blockIdx.x - row * (uint32_t)s.each) * kWaves;
@@ -185,9 +185,9 @@ __device__ __forceinline__ void for_parts(const Shape& s, const int32_t* lengths
     const Sequence q = sequence_of(s, lengths, u.b);
     if (tile > 0 && (int)tile >= q.tiles) return;
     set_unit(s, &u, row - (uint32_t)u.b * s.rows, q, tile, kWaves);
-    if (rows && tile == 0 && threadIdx.x == 0) rows[row] = {blockIdx.x, ((uint32_t)q.tiles + kWaves - 1) / kWaves};
     part(u);
   } else {
+    Row* rows = reinterpret_cast<Row*>(scratch);
     const uint32_t per = share_of(s, lengths);
     uint32_t at = blockIdx.x * per, before;
     if (!find_sequence(s, lengths, at, &u.b, &before)) return;
@@ -640,33 +640,48 @@ __global__ void __launch_bounds__(kWaves * 64, D > 192 ? 1 : 2)
 
 // One workgroup a query head: folds the parts of its row. Lanes take V outputs
 // each, groups of them every G-th part, and the groups are added in order.
-template <typename T, int V>
+template <typename T, int V, bool kAligned>
 __global__ void __launch_bounds__(256)
-    paged_combine(Shape s, const float* __restrict__ scratch, T* __restrict__ out) {
+    paged_combine(Shape s, const int32_t* __restrict__ lengths, const float* __restrict__ scratch,
+                  T* __restrict__ out) {
   __shared__ float f_s[kMaxParts], l_s[kMaxParts];
   __shared__ float red[2][4];
   __shared__ float sums[256 * V];
-  const int64_t b = blockIdx.x / s.p.Hq;
-  const int hq = (int)(blockIdx.x % s.p.Hq);
-  const int kv_head = hq / s.group, ht = (hq % s.group) / kHeads, head = (hq % s.group) % kHeads;
-  const Row row = reinterpret_cast<const Row*>(scratch)[b * s.rows + kv_head * s.head_tiles + ht];
-  if (row.n <= 1) return;
-  const int n = (int)row.n, D = s.p.D;
+  const int64_t b = blockIdx.x / (uint32_t)s.p.Hq;
+  const int hq = (int)(blockIdx.x - (uint32_t)b * (uint32_t)s.p.Hq);
+  const int kv_head = hq / s.group, of_head = hq - kv_head * s.group, head = of_head % kHeads;
+  const int64_t at = b * s.rows + kv_head * s.head_tiles + of_head / kHeads;
+  // The row's first workgroup, and its parts: as many as its keys take, or as
+  // many as there may be, whose states and outputs are requested with the
+  // length that tells.
+  const Row row = kAligned ? Row{(uint32_t)at * (uint32_t)s.each, (uint32_t)s.each}
+                           : reinterpret_cast<const Row*>(scratch)[at];
+  const int D = s.p.D, most = (int)row.n;
+  if (!kAligned && most <= 1) return;
   // Part i's slot: the first starts the row, the others continue it.
   auto part = [&](int i) {
     return slot_state(s, const_cast<float*>(scratch), slot_of((int64_t)row.group + i, i == 0));
   };
-  // The thread's first outputs are requested with the states.
   const int lanes = std::min(256, (D + V - 1) / V), groups = 256 / lanes;
   const int g = threadIdx.x / lanes, lane = threadIdx.x % lanes;
   float first[V];
-  if (g < std::min(groups, n) && lane * V < D)
+  if (g < std::min(groups, most) && lane * V < D)
     __builtin_memcpy(first, part(g) + 2 * s.heads + (int64_t)head * D + lane * V, sizeof(first));
+  float m0 = -INFINITY, l0 = -1.f;
+  if ((int)threadIdx.x < most) {
+    m0 = part(threadIdx.x)[2 * head];
+    l0 = part(threadIdx.x)[2 * head + 1];
+  }
+  int n = most;
+  if constexpr (kAligned) {
+    n = (sequence_of(s, lengths, b).tiles + kWaves - 1) / kWaves;
+    if (n <= 1) return;
+  }
   float m = -INFINITY;
   for (int i = threadIdx.x; i < n; i += 256) {
-    const float* state = part(i) + 2 * head;
-    f_s[i] = state[0];
-    l_s[i] = state[1];
+    const bool here = i == (int)threadIdx.x;
+    f_s[i] = here ? m0 : part(i)[2 * head];
+    l_s[i] = here ? l0 : part(i)[2 * head + 1];
     if (!(l_s[i] < 0.f)) m = fmaxf(m, f_s[i]);
   }
 #pragma unroll
@@ -793,8 +808,13 @@ void launch_paged_attention(hipStream_t stream, const PagedParams& p, DType t, c
 #undef PJRTX_PAGED
     if (!sp) return;
     const dim3 heads(static_cast<uint32_t>(p.B * p.Hq));
-    if (p.D % 4 == 0) hipLaunchKernelGGL((paged_combine<T, 4>), heads, block, 0, stream, s, sp, op);
-    else hipLaunchKernelGGL((paged_combine<T, 1>), heads, block, 0, stream, s, sp, op);
+#define PJRTX_COMBINE(V, ALIGNED) \
+  hipLaunchKernelGGL((paged_combine<T, V, ALIGNED>), heads, block, 0, stream, s, lengths, sp, op)
+    if (p.D % 4 == 0 && s.aligned) PJRTX_COMBINE(4, true);
+    else if (p.D % 4 == 0) PJRTX_COMBINE(4, false);
+    else if (s.aligned) PJRTX_COMBINE(1, true);
+    else PJRTX_COMBINE(1, false);
+#undef PJRTX_COMBINE
   };
   if (t == DType::kF32) go(float());
   else if (t == DType::kBF16) go(bf16_t());
