@@ -220,14 +220,17 @@ __device__ __forceinline__ void for_parts(const Shape& s, const int32_t* lengths
 // of -1 where the wave attended no key, and its outputs are o[(w heads + h) D].
 // Writes the row's results, or the part's, of the unit's heads
 // first .. first + heads - 1.
-template <typename T>
+template <int V, typename T>
 __device__ __forceinline__ void finish_heads(const Shape& s, const Unit& u, int first, int heads,
                                              const float (*ml)[kHeads][2], const float* o, T* out, float* scratch) {
-  const int D = s.p.D;
+  __shared__ float f_s[kWaves][kHeads], l_s[kHeads];
+  const int D = s.p.D, lanes = D / V;
   float* state = u.whole ? nullptr : slot_state(s, scratch, u.slot);
-  for (int i = threadIdx.x; i < heads * D; i += kWaves * 64) {
-    const int h = i / D, d = i - h * D, hu = first + h;
-    float m = -INFINITY;
+  if ((int)threadIdx.x < heads) {
+    // The head's weights of the waves, -1 where a wave's outputs were not
+    // written, and its sum, -1 where none were.
+    const int h = threadIdx.x;
+    float m = -INFINITY, l = 0.f;
     bool any = false;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
@@ -236,23 +239,42 @@ __device__ __forceinline__ void finish_heads(const Shape& s, const Unit& u, int 
       m = none ? m : fmaxf(m, ml[w][h][0]);
     }
     const float ref = m == -INFINITY ? 0.f : m;
-    float l = 0.f, v = 0.f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      if (ml[w][h][1] < 0.f) continue;  // its outputs were not written
-      const float f = exp2f(ml[w][h][0] - ref);
-      l += ml[w][h][1] * f;
-      v += o[(w * heads + h) * D + d] * f;
+      const bool none = ml[w][h][1] < 0.f;
+      const float f = none ? -1.f : exp2f(ml[w][h][0] - ref);
+      f_s[w][h] = f;
+      l += none ? 0.f : ml[w][h][1] * f;
     }
-    if (!state) {
-      out[(u.b * s.p.Hq + u.head0 + hu) * D + d] = (T)(any ? v / l : 0.f);
+    l_s[h] = any ? l : -1.f;
+    if (state) {
+      state[2 * (first + h)] = m;
+      state[2 * (first + h) + 1] = l_s[h];
+    }
+  }
+  __syncthreads();
+  typedef float vec __attribute__((ext_vector_type(V)));
+  typedef T tvec __attribute__((ext_vector_type(V)));
+  typedef vec vec_at __attribute__((aligned(4)));
+  typedef tvec tvec_at __attribute__((aligned(sizeof(T))));
+  for (int i = threadIdx.x; i < heads * lanes; i += kWaves * 64) {
+    const int h = i / lanes, d = (i - h * lanes) * V;
+    vec v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = f_s[w][h];
+      const vec x = *reinterpret_cast<const vec_at*>(o + (w * heads + h) * D + d);
+      if (!(f < 0.f)) v += x * f;
+    }
+    if (state) {
+      *reinterpret_cast<vec_at*>(state + 2 * s.heads + (int64_t)(first + h) * D + d) = v;
       continue;
     }
-    if (d == 0) {
-      state[2 * hu] = m;
-      state[2 * hu + 1] = any ? l : -1.f;
-    }
-    state[2 * s.heads + (int64_t)hu * D + d] = v;
+    const float l = l_s[h];
+    tvec y;
+#pragma unroll
+    for (int e = 0; e < V; ++e) y[e] = (T)(l < 0.f ? 0.f : v[e] / l);
+    *reinterpret_cast<tvec_at*>(out + (u.b * s.p.Hq + u.head0 + first + h) * D + d) = y;
   }
 }
 
@@ -309,7 +331,7 @@ __device__ __forceinline__ void any_part(const Shape& s, const Unit& u, const T*
     for (int j = 0; j < J; ++j)
       if (lane + 64 * j < D) ow[wave * D + lane + 64 * j] = o[j];
     __syncthreads();
-    finish_heads<T>(s, u, h, 1, ml, ow, out, scratch);
+    finish_heads<1>(s, u, h, 1, ml, ow, out, scratch);
     __syncthreads();
   }
 }
@@ -623,7 +645,7 @@ __device__ __forceinline__ void tiles_part(const Shape& s, const Unit& u, const 
       for (int r = 0; r < 4; ++r) ow[(wave * u.heads + c) * D + column_of<T, D>(a, 4 * g + r)] = st.o[a][r];
   }
   __syncthreads();
-  finish_heads<T>(s, u, 0, u.heads, ml, ow, out, scratch);
+  finish_heads<4>(s, u, 0, u.heads, ml, ow, out, scratch);
 }
 
 template <typename T, int D, bool kPage16, bool kAligned>
