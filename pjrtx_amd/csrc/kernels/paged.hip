@@ -1,7 +1,7 @@
 // Attention of one new token a sequence over a paged key-value cache, and the
 // rows that are written into its pages.
 //
-// Work. A row is one sequence with one key-value head and up to 16 of the
+// Work. A row is one sequence with one key-value head and up to 64 of the
 // query heads that share it, so that keys and values are read once for them.
 // The host knows the table's capacity but no length, so the device cuts the
 // work: every workgroup adds the sequences' 32-key tiles (`lengths` is one
@@ -27,11 +27,12 @@ namespace pjrtx {
 namespace {
 
 constexpr int kTileKeys = 32;
-constexpr int kHeads = 16;       // query heads of a row
+constexpr int kHeads = 16;       // query heads of a wave
+constexpr int kSets = 4;         // such sets of a row at most
 constexpr int kRowCost = 4;      // tiles; 0 / 2 / 4 / 8: 115 / 106 / 101 / 102 us at those 64 sequences
 constexpr int kCus = 256;
 constexpr int kMaxParts = 2 * kCus;  // of a row: at most one a workgroup
-constexpr int kWaves = 4;
+constexpr int kWaves = 4, kWavesLog = 2;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // n / d for n < 2^31 by a multiplication (Granlund and Montgomery, 1994).
@@ -51,9 +52,11 @@ __device__ __forceinline__ uint32_t quotient(uint32_t n, const Divisor& v) { ret
 struct Shape {
   PagedParams p;
   int group;       // query heads of a key-value head
-  int head_tiles;  // rows of a (sequence, key-value head)
+  int sets;        // sets of kHeads query heads in a row: 1, 2 or 4,
+  int sets_log;    // 2 to this
+  int head_rows;   // rows of a (sequence, key-value head)
   int heads;       // query heads of a row at most
-  int rows;        // rows of a sequence: Hkv * head_tiles
+  int rows;        // rows of a sequence: Hkv * head_rows
   uint32_t cap;    // keys the table holds, below 2^31
   Divisor page;    // keys of a page
   int groups;      // workgroups of the launch
@@ -161,10 +164,10 @@ struct Unit {
 
 __device__ __forceinline__ void set_unit(const Shape& s, Unit* u, uint32_t r, const Sequence& q, uint32_t tile,
                                          uint32_t n) {
-  const int ht = (int)r % s.head_tiles;
-  u->kv_head = (int)r / s.head_tiles;
-  u->head0 = u->kv_head * s.group + ht * kHeads;
-  u->heads = std::min(kHeads, s.group - ht * kHeads);
+  u->kv_head = (int)r / s.head_rows;
+  const int first = ((int)r - u->kv_head * s.head_rows) * kHeads * s.sets;
+  u->head0 = u->kv_head * s.group + first;
+  u->heads = std::min(kHeads * s.sets, s.group - first);
   u->whole = tile == 0 && (int)n >= q.tiles;
   u->slot = slot_of(blockIdx.x, tile == 0);
   u->lo = q.lo;
@@ -216,35 +219,38 @@ __device__ __forceinline__ void for_parts(const Shape& s, const int32_t* lengths
   }
 }
 
-// The workgroup's waves meet: the state of head h in wave w is ml[w][h], a sum
-// of -1 where the wave attended no key, and its outputs are o[(w heads + h) D].
-// Writes the row's results, or the part's, of the unit's heads
-// first .. first + heads - 1.
-template <int V, typename T>
-__device__ __forceinline__ void finish_heads(const Shape& s, const Unit& u, int first, int heads,
+// The workgroup's waves meet. Wave w holds set w % sets of the heads, for its
+// share of the keys: ml[w][c] is the state of its head c, a sum of -1 where it
+// attended no key, and o[(w slots + c) D] its outputs. Writes the row's results,
+// or the part's, of the unit's heads first .. first + heads - 1.
+template <int V, bool kManySets, typename T>
+__device__ __forceinline__ void finish_heads(const Shape& s, const Unit& u, int first, int heads, int slots,
                                              const float (*ml)[kHeads][2], const float* o, T* out, float* scratch) {
-  __shared__ float f_s[kWaves][kHeads], l_s[kHeads];
+  constexpr int kMost = kManySets ? kSets * kHeads : kHeads;
+  __shared__ float f_s[kWaves][kMost], l_s[kMost];
+  const int sets = kManySets ? s.sets : 1;
   const int D = s.p.D, lanes = D / V;
   float* state = u.whole ? nullptr : slot_state(s, scratch, u.slot);
   if ((int)threadIdx.x < heads) {
     // The head's weights of the waves, -1 where a wave's outputs were not
     // written, and its sum, -1 where none were.
-    const int h = threadIdx.x;
+    const int h = threadIdx.x, c = kManySets ? h % kHeads : h;
+    auto none_of = [&](int w) { return (kManySets && (w & (sets - 1)) != h / kHeads) || ml[w][c][1] < 0.f; };
     float m = -INFINITY, l = 0.f;
     bool any = false;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const bool none = ml[w][h][1] < 0.f;
+      const bool none = none_of(w);
       any = any || !none;
-      m = none ? m : fmaxf(m, ml[w][h][0]);
+      m = none ? m : fmaxf(m, ml[w][c][0]);
     }
     const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const bool none = ml[w][h][1] < 0.f;
-      const float f = none ? -1.f : exp2f(ml[w][h][0] - ref);
+      const bool none = none_of(w);
+      const float f = none ? -1.f : exp2f(ml[w][c][0] - ref);
       f_s[w][h] = f;
-      l += none ? 0.f : ml[w][h][1] * f;
+      l += none ? 0.f : ml[w][c][1] * f;
     }
     l_s[h] = any ? l : -1.f;
     if (state) {
@@ -263,7 +269,7 @@ __device__ __forceinline__ void finish_heads(const Shape& s, const Unit& u, int 
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       const float f = f_s[w][h];
-      const vec x = *reinterpret_cast<const vec_at*>(o + (w * heads + h) * D + d);
+      const vec x = *reinterpret_cast<const vec_at*>(o + (w * slots + (kManySets ? h % kHeads : h)) * D + d);
       if (!(f < 0.f)) v += x * f;
     }
     if (state) {
@@ -331,7 +337,7 @@ __device__ __forceinline__ void any_part(const Shape& s, const Unit& u, const T*
     for (int j = 0; j < J; ++j)
       if (lane + 64 * j < D) ow[wave * D + lane + 64 * j] = o[j];
     __syncthreads();
-    finish_heads<1>(s, u, h, 1, ml, ow, out, scratch);
+    finish_heads<1, false>(s, u, h, 1, 1, ml, ow, out, scratch);
     __syncthreads();
   }
 }
@@ -349,7 +355,7 @@ __global__ void __launch_bounds__(kWaves * 64)
 
 // ------------------------------------------------------------------- tiles
 // Head dims that are whole matrix steps. A wave takes 32 keys at a time (16 in
-// f32) for all the row's heads: S^T = K.Q^T with the keys as the matrix rows
+// f32) for its heads: S^T = K.Q^T with the keys as the matrix rows
 // and the heads as its 16 columns, so a lane holds scores of one head (its
 // column, lane & 15) for keys 4g + r of each 16 (g = lane / 16), and these are,
 // as they lie, the right operand of O^T += V^T.P^T. K goes from memory to the
@@ -584,7 +590,7 @@ __device__ __forceinline__ void use_tile(float scale2, Tile<T, D>& t, Heads<T, D
   }
 }
 
-template <typename T, int D, bool kPage16>
+template <typename T, int D, bool kPage16, bool kManySets>
 __device__ __forceinline__ void tiles_part(const Shape& s, const Unit& u, const T* __restrict__ q,
                                            const T* __restrict__ k_pages, const T* __restrict__ v_pages,
                                            const int32_t* __restrict__ table, T* __restrict__ out, float* scratch,
@@ -592,6 +598,11 @@ __device__ __forceinline__ void tiles_part(const Shape& s, const Unit& u, const 
   using Sh = TileShape<T, D>;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // The wave's heads, and its share of the keys beside the other waves of the
+  // set. (The sets' waves read a tile about at once: it comes from HBM once.)
+  const int log = kManySets ? s.sets_log : 0, key_waves = kWaves >> log, key_wave = wave >> log;
+  const int head0 = kManySets ? (wave & (s.sets - 1)) * kHeads : 0;
+  const int heads = std::min(kHeads, u.heads - head0), slots = std::min(kHeads, u.heads);
   Heads<T, D> st;
   st.m = -INFINITY;
   st.l = 0.f;
@@ -599,19 +610,20 @@ __device__ __forceinline__ void tiles_part(const Shape& s, const Unit& u, const 
   st.seen = 0;
 #pragma unroll
   for (int a = 0; a < Sh::kAcc; ++a) st.o[a] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const T* qr = q + (u.b * s.p.Hq + u.head0 + std::min(c, u.heads - 1)) * D;
+  const T* qr = q + (u.b * s.p.Hq + u.head0 + std::min(head0 + c, u.heads - 1)) * D;
 #pragma unroll
   for (int i = 0; i < Sh::kKWords / 4; ++i) {
     load_words<4>(qr + (4 * i + g) * (16 / (int)sizeof(T)), st.q + 4 * i);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) st.q[4 * i + e] = c < u.heads ? st.q[4 * i + e] : 0u;
+    for (int e = 0; e < 4; ++e) st.q[4 * i + e] = c < heads ? st.q[4 * i + e] : 0u;
   }
   const float scale2 = s.p.scale * kLog2e;
-  // Step i of the wave: its tiles are every kWaves-th from tile0 + wave.
+  // Step i of the wave: its tiles are every key_waves-th from tile0 + key_wave.
   constexpr int kSteps = kTileKeys / Sh::kKeys;
-  const int steps = u.tile0 + wave < u.tile1 ? ((u.tile1 - u.tile0 - wave + kWaves - 1) / kWaves) * kSteps : 0;
+  const int tiles = u.tile1 - u.tile0 - key_wave;
+  const int steps = heads > 0 && tiles > 0 ? ((tiles + key_waves - 1) >> (kWavesLog - log)) * kSteps : 0;
   auto key_of = [&](int i) {
-    return (uint32_t)(u.tile0 + wave + i / kSteps * kWaves) * kTileKeys + i % kSteps * Sh::kKeys;
+    return (uint32_t)(u.tile0 + key_wave + i / kSteps * key_waves) * kTileKeys + i % kSteps * Sh::kKeys;
   };
   if (steps > 0) {
     Tile<T, D> t;
@@ -634,29 +646,29 @@ __device__ __forceinline__ void tiles_part(const Shape& s, const Unit& u, const 
   float l = st.l4[0];
   if constexpr (!Sh::kHalf) l = st.l + __shfl_xor(st.l, 16), l += __shfl_xor(l, 32);
   const bool any = __any(st.seen != 0);
-  if (lane < u.heads) {
+  if (lane < heads) {
     ml[wave][lane][0] = st.m;
     ml[wave][lane][1] = any ? l : -1.f;
   }
-  if (any && c < u.heads) {
+  if (any && c < heads) {
 #pragma unroll
     for (int a = 0; a < Sh::kAcc; ++a)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) ow[(wave * u.heads + c) * D + column_of<T, D>(a, 4 * g + r)] = st.o[a][r];
+      for (int r = 0; r < 4; ++r) ow[(wave * slots + c) * D + column_of<T, D>(a, 4 * g + r)] = st.o[a][r];
   }
   __syncthreads();
-  finish_heads<4>(s, u, 0, u.heads, ml, ow, out, scratch);
+  finish_heads<4, kManySets>(s, u, 0, u.heads, slots, ml, ow, out, scratch);
 }
 
-template <typename T, int D, bool kPage16, bool kAligned>
+template <typename T, int D, bool kPage16, bool kAligned, bool kManySets>
 __global__ void __launch_bounds__(kWaves * 64, D > 192 ? 1 : 2)
     paged_tiles(Shape s, const T* __restrict__ q, const T* __restrict__ k_pages, const T* __restrict__ v_pages,
                 const int32_t* __restrict__ table, const int32_t* __restrict__ lengths, T* __restrict__ out,
                 float* __restrict__ scratch) {
   __shared__ float ml[kWaves][kHeads][2];
-  extern __shared__ float ow[];  // [waves][heads][D]
+  extern __shared__ float ow[];  // [waves][heads of a wave][D]
   for_parts<kAligned>(s, lengths, scratch, [&](const Unit& u) {
-    tiles_part<T, D, kPage16>(s, u, q, k_pages, v_pages, table, out, scratch, ml, ow);
+    tiles_part<T, D, kPage16, kManySets>(s, u, q, k_pages, v_pages, table, out, scratch, ml, ow);
   });
 }
 
@@ -671,8 +683,8 @@ __global__ void __launch_bounds__(256)
   __shared__ float sums[256 * V];
   const int64_t b = blockIdx.x / (uint32_t)s.p.Hq;
   const int hq = (int)(blockIdx.x - (uint32_t)b * (uint32_t)s.p.Hq);
-  const int kv_head = hq / s.group, of_head = hq - kv_head * s.group, head = of_head % kHeads;
-  const int64_t at = b * s.rows + kv_head * s.head_tiles + of_head / kHeads;
+  const int kv_head = hq / s.group, of_head = hq - kv_head * s.group, head = of_head % (kHeads * s.sets);
+  const int64_t at = b * s.rows + kv_head * s.head_rows + of_head / (kHeads * s.sets);
   // The row's first workgroup, and its parts: as many as its keys take, or as
   // many as there may be, whose states and outputs are requested with the
   // length that tells.
@@ -758,20 +770,27 @@ __global__ void __launch_bounds__(256)
 // leave, so that a launch's workgroups run at once.
 int groups_per_cu(const PagedParams& p) { return p.D > 192 ? 1 : 2; }
 
+// Head dims that paged_tiles takes.
+bool takes_tiles(int D) { return D == 32 || D == 64 || D == 96 || D == 128 || D == 192 || D == 256; }
+
 Shape shape_of(const PagedParams& p) {
   Shape s;
   s.p = p;
   s.group = p.Hq / p.Hkv;
-  s.head_tiles = (s.group + kHeads - 1) / kHeads;
-  s.heads = std::min(s.group, kHeads);
-  s.rows = p.Hkv * s.head_tiles;
+  // 8 sequences of 8192 keys, 8 heads of 128 with 32 query heads each, bf16:
+  // 90 us in rows of 16, 74 in rows of 32.
+  s.sets = s.group <= kHeads || !takes_tiles(p.D) ? 1 : s.group <= 2 * kHeads ? 2 : kSets;
+  s.sets_log = s.sets / 2;
+  s.heads = std::min(s.group, kHeads * s.sets);
+  s.head_rows = (s.group + kHeads * s.sets - 1) / (kHeads * s.sets);
+  s.rows = p.Hkv * s.head_rows;
   s.cap = static_cast<uint32_t>(p.M * p.S);
   s.page = divisor_of(static_cast<uint32_t>(p.S));
   // The table's tiles as workgroups of one tile a wave, row by row: where they
   // are no more than run at once, that is the launch.
   const int64_t tiles = (static_cast<int64_t>(s.cap) + kTileKeys - 1) / kTileKeys;
   const int64_t each = (tiles + kWaves - 1) / kWaves, most = kCus * groups_per_cu(p);
-  s.aligned = p.B * s.rows * each <= most;
+  s.aligned = s.sets == 1 && p.B * s.rows * each <= most;
   s.each = static_cast<int>(each);
   s.groups = static_cast<int>(s.aligned ? p.B * s.rows * each : most);
   return s;
@@ -806,14 +825,18 @@ void launch_paged_attention(hipStream_t stream, const PagedParams& p, DType t, c
     float* sp = static_cast<float*>(scratch);
 #define PJRTX_PAGED_AS(...) \
   hipLaunchKernelGGL((__VA_ARGS__), grid, block, lds, stream, s, qp, kp, vp, page_table, lengths, op, sp)
-#define PJRTX_PAGED(DIM)                                                         \
-  case DIM:                                                                      \
-    if (p.S % 16 == 0 && s.aligned) PJRTX_PAGED_AS(paged_tiles<T, DIM, true, true>);   \
-    else if (p.S % 16 == 0) PJRTX_PAGED_AS(paged_tiles<T, DIM, true, false>);    \
-    else if (s.aligned) PJRTX_PAGED_AS(paged_tiles<T, DIM, false, true>);        \
-    else PJRTX_PAGED_AS(paged_tiles<T, DIM, false, false>);                      \
+#define PJRTX_PAGED_PAGES(DIM, ALIGNED, SETS)                                       \
+  do {                                                                              \
+    if (p.S % 16 == 0) PJRTX_PAGED_AS(paged_tiles<T, DIM, true, ALIGNED, SETS>);    \
+    else PJRTX_PAGED_AS(paged_tiles<T, DIM, false, ALIGNED, SETS>);                 \
+  } while (0)
+#define PJRTX_PAGED(DIM)                                         \
+  case DIM:                                                      \
+    if (s.sets > 1) PJRTX_PAGED_PAGES(DIM, false, true);         \
+    else if (s.aligned) PJRTX_PAGED_PAGES(DIM, true, false);     \
+    else PJRTX_PAGED_PAGES(DIM, false, false);                   \
     break
-    size_t lds = static_cast<size_t>(kWaves) * s.heads * p.D * sizeof(float);  // the waves' outputs
+    size_t lds = static_cast<size_t>(kWaves) * std::min(s.heads, kHeads) * p.D * sizeof(float);  // the waves' outputs
     switch (p.D) {
       PJRTX_PAGED(32);
       PJRTX_PAGED(64);
@@ -827,6 +850,7 @@ void launch_paged_attention(hipStream_t stream, const PagedParams& p, DType t, c
         else PJRTX_PAGED_AS(paged_any<T, false>);
     }
 #undef PJRTX_PAGED_AS
+#undef PJRTX_PAGED_PAGES
 #undef PJRTX_PAGED
     if (!sp) return;
     const dim3 heads(static_cast<uint32_t>(p.B * p.Hq));

@@ -111,7 +111,7 @@ LENGTHS = [1, 0, 2, 31, 32, 33, 127, 129, 300]
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("kv_heads,group,dim,size", [
     (2, 1, 128, 16), (2, 4, 64, 16), (1, 8, 128, 32), (3, 5, 96, 24), (1, 16, 64, 8), (1, 33, 128, 16), (2, 2, 256, 1),
-    (1, 2, 192, 48), (1, 16, 256, 16), (1, 17, 192, 24), (2, 3, 32, 16), (1, 9, 32, 4), (2, 3, 80, 7), (1, 1, 1, 5), (1, 2, 500, 16), (1, 3, 33, 130)])
+    (1, 2, 192, 48), (1, 16, 256, 16), (1, 17, 192, 24), (2, 3, 32, 16), (1, 9, 32, 4), (2, 40, 64, 16), (1, 70, 96, 12), (1, 32, 256, 16), (2, 3, 80, 7), (1, 1, 1, 5), (1, 2, 500, 16), (1, 3, 33, 130)])
 def test_paged_attention_shapes(client, dtype, kv_heads, group, dim, size):
     rng = np.random.default_rng(dim * 7 + size)
     k, v, table = cache(rng, LENGTHS, kv_heads, size, dim, dtype)
@@ -195,7 +195,7 @@ def test_paged_attention_infinities(client, dtype, dim):
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("lengths", [[5000], [3000, 1, 0, 17], [700] * 9 + [2500], [64] * 300, [1] * 70 + [900] * 3])
-@pytest.mark.parametrize("group,dim", [(4, 128), (20, 64), (2, 72)])
+@pytest.mark.parametrize("group,dim", [(4, 128), (20, 64), (50, 32), (2, 72)])
 def test_paged_attention_split_lengths(client, dtype, lengths, group, dim):
     """Long sequences cut into splits, many sequences, both beside short ones."""
     rng = np.random.default_rng(len(lengths))
