@@ -129,11 +129,13 @@ __device__ __forceinline__ bool find_sequence(const Shape& s, const int32_t* len
 }
 
 // Key j's row of the pages (in rows of D elements), -1 where the table's entry
-// names no page. j is clamped to the table; the pages have fewer than 2^31 rows.
+// names no page or j is past the table, as the keys of a last tile may be: its
+// entry is read all the same, clamped, so that the read waits for no length.
+// The pages have fewer than 2^31 rows.
 __device__ __forceinline__ int row_of(const Shape& s, const int32_t* table, int64_t b, int kv_head, uint32_t j) {
   const uint32_t e = std::min(quotient(j, s.page), (uint32_t)s.p.M - 1);
   const int page = table[b * s.p.M + e];
-  if (page < 0 || page >= s.p.P) return -1;
+  if (page < 0 || page >= s.p.P || j >= s.cap) return -1;
   return (page * s.p.Hkv + kv_head) * (int)s.page.d + (int)(j - e * s.page.d);
 }
 
@@ -970,8 +972,7 @@ void launch_paged_append(hipStream_t s, const AppendParams& p, int elem_bytes, v
   // The widest unit that every row starts on.
   if (addresses % 16 == 0) go(uint4());
   else if (addresses % 4 == 0) go(uint32_t());
-  else if (addresses % 2 == 0) go(uint16_t());
-  else go(uint8_t());
+  else go(uint16_t());
   check_launch("paged_append");
 }
 

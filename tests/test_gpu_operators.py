@@ -216,6 +216,21 @@ def test_paged_attention_results_do_not_depend_on_the_pages_order(client):
     assert np.array_equal(got, attend(client, q, k[perm], v[perm], moved, [700, 90], "bf16"))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("size,dim", [(8, 64), (16, 128), (48, 64), (5, 96), (7, 40)])
+def test_paged_attention_full_tables_at_the_pools_end(client, dtype, size, dim):
+    """Sequences that fill their table, the last page the pool's last, with
+    tables that end inside a 32-key tile."""
+    rng = np.random.default_rng(size)
+    for width in (1, 3, 11):
+        pages, n = 2 * width, width * size
+        k, v = (put(x, dtype) for x in rng.standard_normal((2, pages, 1, size, dim)))
+        table = np.stack([rng.permutation(width), width + np.arange(width)]).astype(np.int32)
+        q = put(rng.standard_normal((2, 3, dim)), dtype)
+        attend(client, q, k, v, table, [n, n], dtype)
+        attend(client, q, k, v, table, [n - 1, 2 ** 31 - 1], dtype, window=max(1, n // 2))
+
+
 def test_paged_attention_rows_past_32_bits(client):
     """Pages of more than 2^32 bytes, written and read at their end."""
     pages, size, dim = 140000, 64, 256
@@ -554,3 +569,89 @@ def test_token_logprobs_grad_is_the_forward_passs_difference(client):
             e = np.zeros_like(x)
             e[r, i] = s
             assert abs((loss(x + e) - loss(x - e)) / (2 * s) - dx[r, i]) < 10 * s * s
+
+
+# ---------------------------------------------------- the caller's addresses
+
+def _off(client, a, by):
+    """Device memory that holds `a` from `by` bytes on."""
+    raw = np.zeros(a.nbytes + by, np.uint8)
+    raw[by:] = np.ascontiguousarray(a).view(np.uint8).ravel()
+    return DeviceArray.from_numpy(client.p, raw)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("what", ["attention", "any", "append", "norm", "quantized", "norm_grad", "long_grad", "logprobs",
+                                  "logprobs_grad"])
+def test_addresses_are_an_elements(client, dtype, what):
+    """Arguments and outputs at any element's address: the bits of aligned ones."""
+    rng = np.random.default_rng(12)
+    r = lambda *shape: put(rng.standard_normal(shape), dtype)  # noqa: E731
+    ints = lambda *v: np.array(v, np.int32)  # noqa: E731
+    f = lambda n: rng.standard_normal(n).astype(np.float32)  # noqa: E731
+    table = np.array([[3, 1, 0, 2], [2, 0, 3, -1]], np.int32)
+    dim = 64 if what == "attention" else 40
+    args, build = {
+        "attention": ([r(2, 6, dim), r(4, 2, 16, dim), r(4, 2, 16, dim), table, ints(60, 33)], lambda b, p: [b.paged_attention(*p)]),
+        "any": ([r(2, 6, dim), r(4, 2, 16, dim), r(4, 2, 16, dim), table, ints(60, 33)], lambda b, p: [b.paged_attention(*p)]),
+        "append": ([r(4, 2, 16, 32), r(4, 2, 16, 32), r(5, 2, 32), r(5, 2, 32), ints(3, 9, 3, 60, -1)],
+                   lambda b, p: b.paged_append(*p)),
+        "norm": ([r(5, 1032), r(5, 1032), r(1032)], lambda b, p: b.add_rms_norm(*p)),
+        "quantized": ([r(5, 1032), r(5, 1032), r(1032)], lambda b, p: b.add_rms_norm(*p, quantize=True)),
+        "norm_grad": ([r(9, 520), r(9, 520), r(9, 520), r(520)], lambda b, p: b.add_rms_norm_grad(*p)),
+        "long_grad": ([r(3, 9000), r(3, 9000), r(3, 9000), r(9000)], lambda b, p: b.add_rms_norm_grad(*p)),
+        "logprobs": ([r(3, 9000), ints(1, 2, 3)], lambda b, p: b.token_logprobs(*p, top_k=7)),
+        "logprobs_grad": ([r(3, 9000), ints(1, 2, 3), f(3) + 9, f(3), f(3), f(3)], lambda b, p: [b.token_logprobs_grad(*p)]),
+    }[what]
+    names = {np.dtype(np.uint16): "bf16", np.dtype(np.float32): "f32", np.dtype(np.int32): "s32"}
+    b = Builder()
+    exe = client.compile(b.build(list(build(b, [b.param(a.shape, names[a.dtype]) for a in args]))))
+    want = exe(*args, dtypes=["bf16" if a.dtype == np.uint16 else None for a in args])
+    size = 2 if dtype == "bf16" else 4
+    for by in (size, 3 * size):
+        ins = [_off(client, a, by * a.dtype.itemsize // size) for a in args]
+        outs = [DeviceArray(client.p, w.nbytes + by * w.dtype.itemsize // size) for w in want]
+        exe.execute_noalloc([d.ptr + by * a.dtype.itemsize // size for d, a in zip(ins, args)],
+                            [d.ptr + by * w.dtype.itemsize // size for d, w in zip(outs, want)])
+        client.p.hip_check(client.p.lib.pjrtx_hip_synchronize(0))
+        for d, w in zip(outs, want):
+            at = by * w.dtype.itemsize // size
+            got = d.to_numpy(np.uint8, (w.nbytes + at,))[at:]
+            assert np.array_equal(got, w.view(np.uint8).ravel())
+        for d in ins + outs:
+            d.free()
+
+
+# ------------------------------------------------------------ inside a loop
+
+def test_append_and_attention_inside_a_while_loop(client):
+    """Steps of a decode loop on the device: each appends a row and attends."""
+    rng = np.random.default_rng(13)
+    steps, dim = 20, 64
+    k, v = (put(x, "bf16") for x in rng.standard_normal((2, 6, 2, 8, dim)))
+    table = np.array([[4, 1, 5, 0, 2, 3]], np.int32)
+    rows = put(rng.standard_normal((steps, 2, dim)), "bf16")
+    q = put(rng.standard_normal((1, 4, dim)), "bf16")
+    b = Builder()
+    kp, vp = b.param(k.shape, "bf16", donate=True), b.param(v.shape, "bf16", donate=True)
+    tb, rp, qp = b.param(table.shape, "s32"), b.param(rows.shape, "bf16"), b.param(q.shape, "bf16")
+    n, size, one, zero = b.constant(steps, "s32"), b.constant(8, "s32"), b.constant(1, "s32"), b.constant(0, "s32")
+    outs = b.broadcast_in_dim(b.constant(0.0, "bf16"), (steps, 4, dim), [])
+
+    def body(i, kc, vc, o):
+        row = b.dynamic_slice(rp, [i, zero, zero], (1, 2, dim))
+        page = b.dynamic_slice(tb, [zero, b.divide(i, size)], (1, 1))
+        slot = b.add(b.multiply(b.reshape(page, ()), size), b.remainder(i, size))
+        kc, vc = b.paged_append(kc, vc, row, row, b.reshape(slot, (1,)))
+        a = b.paged_attention(qp, kc, vc, tb, b.reshape(b.add(i, one), (1,)))
+        return [b.add(i, one), kc, vc, b.dynamic_update_slice(o, a, [i, zero, zero])]
+
+    end = b.while_loop([zero, kp, vp, outs], lambda i, *_: b.compare("LT", i, n), body)
+    got_k, got_v, got = client.compile(b.build([end[1], end[2], end[3]]))(k, v, table, rows, q,
+                                                                          dtypes=["bf16", "bf16", None, "bf16", "bf16"])
+    slots = np.array([table[0, i // 8] * 8 + i % 8 for i in range(steps)])
+    wk, wv = P.paged_append(k, v, rows, rows, slots)
+    assert np.array_equal(got_k, wk) and np.array_equal(got_v, wv)
+    for i in range(steps):
+        want = P.paged_attention(val(q), val(wk), val(wv), table, [i + 1])
+        close(got[i:i + 1], want, attention_tolerance(q, wk, wv, want, "bf16", dim ** -0.5, i + 1))
