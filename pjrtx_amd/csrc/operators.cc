@@ -57,7 +57,9 @@ class Checker {
     if (it == op_.config.end()) return dflt;
     char* end = nullptr;
     const double v = std::strtod(it->second.c_str(), &end);
-    need(end != it->second.c_str() && at_type(end), std::string(key) + " must be a number");
+    // MLIR writes infinities and NaNs as hexadecimal bits.
+    const bool bits = it->second.find_first_of("xX") < it->second.find(':');
+    need(end != it->second.c_str() && at_type(end) && !bits, std::string(key) + " must be a finite number");
     return v;
   }
   int64_t integer(const char* key, int64_t dflt) const {
@@ -259,6 +261,29 @@ LibKind operator_lib_kind(OpKind k) {
     case OpKind::kTokenLogprobsGrad: return LibKind::kTokenLogprobsGrad;
     default: return LibKind::kCopy;
   }
+}
+
+double operator_bytes(const Program& prog, const Step& step) {
+  const Op& op = prog.ops.at(step.lib_op);
+  double bytes = 0;
+  for (size_t i = 0; i < op.operands.size(); ++i) {
+    const bool pages = (op.kind == OpKind::kPagedAttention && (i == 1 || i == 2)) ||
+                       (op.kind == OpKind::kPagedAppend && i < 2);
+    if (!pages) bytes += static_cast<double>(prog.type(op.operands[i]).bytes());
+  }
+  if (op.kind == OpKind::kPagedAppend) {
+    bytes += static_cast<double>(prog.type(op.operands[2]).bytes() + prog.type(op.operands[3]).bytes());
+    for (int k = 0; k < 2; ++k)
+      if (!(step.in_place_operands & (1u << k))) bytes += 2.0 * static_cast<double>(prog.type(op.operands[k]).bytes());
+    return bytes;
+  }
+  for (int v : op.results) bytes += static_cast<double>(prog.type(v).bytes());
+  if (op.kind == OpKind::kPagedAttention) {
+    const TensorType& k = prog.type(op.operands[1]);
+    const double named = static_cast<double>(prog.type(op.operands[3]).elements()) / static_cast<double>(k.dims[0]);
+    bytes += 2.0 * std::min(named, 1.0) * static_cast<double>(k.bytes());
+  }
+  return bytes;
 }
 
 void run_operator(Device* dev, const Program& prog, const Step& step, std::vector<MemRef>& vals) {

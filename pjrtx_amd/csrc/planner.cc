@@ -1418,12 +1418,8 @@ std::string Plan::describe(const Program& prog) const {
       } else if (s.lib == LibKind::kDynamicUpdateSlice && s.in_place) {
         alg = 2 * prog.type(d.operands[1]).bytes();
         for (size_t k = 2; k < d.operands.size(); ++k) alg += prog.type(d.operands[k]).bytes();
-      } else if (s.lib == LibKind::kPagedAppend) {
-        // The new rows read and written; pages that are not written in place
-        // are copied.
-        alg = 2 * (prog.type(d.operands[2]).bytes() + prog.type(d.operands[3]).bytes()) + prog.type(d.operands[4]).bytes();
-        for (int k = 0; k < 2; ++k)
-          if (!(s.in_place_operands & (1u << k))) alg += 2 * prog.type(d.operands[k]).bytes();
+      } else if (operator_lib_kind(d.kind) != LibKind::kCopy) {
+        alg = static_cast<int64_t>(operator_bytes(prog, s));
       }
     }
     if (s.kind == StepKind::kGemv) {

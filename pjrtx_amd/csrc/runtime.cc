@@ -1279,6 +1279,10 @@ bool Executable::graph_candidate(const std::vector<BufferRef>& args, const std::
     for (const Step& st : plan_.steps) {
       if (st.kind == StepKind::kAlias) continue;
       ++n;
+      if (st.kind == StepKind::kLibrary && operator_lib_kind(prog_.ops[st.lib_op].kind) != LibKind::kCopy) {
+        bytes += operator_bytes(prog_, st);
+        continue;
+      }
       for (int v : st.inputs) bytes += static_cast<double>(prog_.type(v).bytes());
       for (size_t k = 0; k < st.outputs.size(); ++k) {
         auto ww = st.window_out.find(static_cast<int>(k));

@@ -78,7 +78,7 @@ LOG, LGRAD = "pjrtx.token_logprobs", "pjrtx.token_logprobs_grad"
     bad(ATT, 1, (8, 2, 16, 32)), bad(ATT, 2, dtype="f16"), bad(ATT, 2, (8, 2, 8, 64)), bad(ATT, 3, dtype="s64"),
     bad(ATT, 3, (2, 5)), bad(ATT, 3, (3, 0)), bad(ATT, 4, (4,)), bad(ATT, 4, dtype="u32"),
     bad(ATT, result=(0, (3, 4, 64), "f32")), bad(ATT, config={"window": -1}), bad(ATT, config={"soft_cap": 1.0}),
-    bad(ATT, config={"scale": float("inf")}), bad(ATT, 3, (3, 1 << 27), code=UNIMPLEMENTED),
+    bad(ATT, config={"scale": float("inf")}), bad(ATT, config={"scale": float("nan")}), bad(ATT, 3, (3, 1 << 27), code=UNIMPLEMENTED),
     bad(APP, drop=4), bad(APP, 2, (7, 3, 64)), bad(APP, 3, (6, 2, 64)), bad(APP, 4, (6,)), bad(APP, 4, dtype="u32"),
     bad(APP, 3, dtype="f32"), bad(APP, result=(1, PAGES, "f32")), bad(APP, drop_result=True), bad(APP, config={"page": 16}),
     bad(NORM, 1, (3, 5, 64)), bad(NORM, 2, (64,)), bad(NORM, 2, dtype="f16"), bad(NORM, 0, dtype="s32"),
@@ -152,3 +152,35 @@ def test_pages_read_later_are_kept(plugin):
         later = [v for t in p["steps"][i + 1:] for v in t["inputs"]]
         for k in range(2):
             assert not (s["in_place_operands"] >> k & 1) or s["inputs"][k] not in later
+
+
+def test_attributes_as_jax_prints_them(plugin):
+    """Hexadecimal bits are infinities and NaNs; layouts, aliases and unknown
+    attributes of the call itself are not the operator's."""
+    ins, outs = CALLS[ATT]
+    text = text_of(ATT, ins, outs, {"scale": 0.25, "window": 7})
+    assert len(plan(plugin, text)["steps"]) == 1
+    for value in ("0x7F800000 : f32", "0xFFC00000 : f32", "true", '"1.0"', "[1.0]", "1.0.0 : f32"):
+        with pytest.raises(PjrtError) as e:
+            plan(plugin, text.replace("2.50000000000000000e-01 : f64", value))
+        assert e.value.code == INVALID and "scale" in e.value.message
+    for value in ("9.99999974E-6 : f32", "1 : i64", "0.5", "-2.0e+00 : f64"):
+        assert plan(plugin, text.replace("2.50000000000000000e-01 : f64", value))["steps"]
+    ins, outs = CALLS[APP]
+    text = text_of(APP, ins, outs).replace(
+        "backend_config = {}", "backend_config = {}, has_side_effect = false, operand_layouts = [dense<[3, 2, 1, 0]> : "
+        "tensor<4xindex>, dense<[3, 2, 1, 0]> : tensor<4xindex>], output_operand_aliases = "
+        "[#stablehlo.output_operand_alias<output_tuple_indices = [0], operand_index = 0, operand_tuple_indices = []>]")
+    assert plan(plugin, text)["steps"][0]["library"] == "paged_append"
+
+
+def test_bytes_of_a_step_are_those_it_moves(plugin):
+    """Of a cache's pages, the rows named; the whole pages where they are copied."""
+    ins, outs = CALLS[ATT]
+    big = [((1000, 2, 16, 64), "bf16") if t[0] == PAGES else t for t in ins]
+    step = plan(plugin, text_of(ATT, big, outs))["steps"][0]
+    assert step["algorithmic_bytes"] == 2 * 3 * 4 * 64 * 2 + 4 * 15 + 4 * 3 + 2 * 15 * 2 * 16 * 64 * 2
+    step = plan(plugin, _append(True))["steps"][0]
+    assert step["algorithmic_bytes"] == 4 * 7 * 2 * 64 * 2 + 4 * 7
+    step = plan(plugin, _append(False))["steps"][0]
+    assert step["algorithmic_bytes"] == 4 * 7 * 2 * 64 * 2 + 4 * 7 + 4 * 8 * 2 * 16 * 64 * 2
