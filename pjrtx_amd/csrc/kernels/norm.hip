@@ -43,7 +43,8 @@ __device__ __forceinline__ float row_max_nan(float x, float* red) {
 }
 
 // y over the row's scale, rounded to the nearest even; NaN counts as 0 (its
-// scale is NaN, so what it stands for stays NaN).
+// scale is NaN, so what it stands for stays NaN). Under an infinite scale an
+// infinite y is +-127, which stands for itself.
 struct Quant {
   float scale, inv;
   bool divide;
@@ -52,12 +53,12 @@ __device__ __forceinline__ Quant quant_of(float amax) {
   Quant q;
   q.scale = amax / 127.f;
   // The reciprocal of a scale below 2^-120 could overflow: those rows divide.
-  q.divide = !(q.scale >= 0x1p-120f);
+  q.divide = !(q.scale >= 0x1p-120f && q.scale < HUGE_VALF);
   q.inv = q.divide ? 0.f : 1.f / q.scale;
   return q;
 }
 __device__ __forceinline__ int8_t quantize(float y, const Quant& q) {
-  float v = q.divide ? (q.scale > 0.f ? y / q.scale : 0.f) : y * q.inv;
+  float v = q.divide ? (fabsf(y) == HUGE_VALF ? y : q.scale > 0.f ? y / q.scale : 0.f) : y * q.inv;
   v = fminf(fmaxf(rintf(v), -127.f), 127.f);  // fmaxf(NaN, -127) is -127
   return y == y ? (int8_t)v : (int8_t)0;
 }

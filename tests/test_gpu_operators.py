@@ -378,6 +378,18 @@ def test_add_rms_norm_not_finite(client, dtype):
     assert np.isnan(scale[1:]).all() and scale[0] > 0 and (y8[0] == 127).all()
 
 
+def test_add_rms_norm_infinite_gain_quantizes(client):
+    """An infinite scale: +-127 stand for the infinities, 0 for what no value
+    stands for."""
+    x = np.full((2, 300), -1.0, np.float32)
+    x[1, 5] = 0
+    g = np.ones(300, np.float32)
+    g[5], g[9] = np.inf, -np.inf
+    y8, scale = call(client, lambda b, p: b.add_rms_norm(p[0], None, p[1], quantize=True), [x, g], ["f32"] * 2)
+    assert scale[0] == np.inf and np.isnan(scale[1])
+    assert y8[0, 5] == -127 and y8[0, 9] == 127 and not np.delete(y8[0], [5, 9]).any()
+
+
 def test_add_rms_norm_small_rows_quantize(client):
     """Scales near the smallest floats: the quotients stay finite."""
     x = np.zeros((4, 64), np.float32)
