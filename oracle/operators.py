@@ -65,11 +65,11 @@ def token_logprobs(logits, tokens, top_k=0):
     entropy = np.log(z) - (e * d).sum(1) / z
     rows = np.arange(logits.shape[0])
     known = (tokens >= 0) & (tokens < logits.shape[1])
-    lp = np.where(known, logits[rows, np.where(known, tokens, 0)] - lse, 0.0)
+    lp = np.where(known, (logits[rows, np.where(known, tokens, 0)] - m[:, 0]) - np.log(z), 0.0)
     if not top_k:
         return lp, entropy, lse
     ids = np.argsort(-logits, axis=1, kind="stable")[:, :top_k]
-    return lp, entropy, lse, logits[rows[:, None], ids] - lse[:, None], ids
+    return lp, entropy, lse, (logits[rows[:, None], ids] - m) - np.log(z)[:, None], ids
 
 
 def token_logprobs_grad(logits, tokens, lse, entropy, d_lp, d_entropy):

@@ -2,12 +2,11 @@
 // likeliest tokens, in one pass over the logits; and their gradient.
 //
 // A row is split over workgroups, which read it in chunks of 8192 elements
-// held in registers. Each thread keeps an online softmax of its own, in powers
-// of two: m = x log2(e) of the largest x so far, l = sum 2^y and a = sum 2^y y
-// with y = x log2(e) - m, from which lse = (m + log2 l) ln 2 and entropy =
-// (log2 l - a / l) ln 2. The entropy's terms are taken about m, not about zero,
-// so nothing large cancels, and m is the number that is subtracted, so its own
-// rounding is in no result. Elements that may be among the
+// held in registers. Each thread keeps an online softmax of its own: m, the
+// largest x so far, l = sum e^d and a = sum e^d d with d = x - m, from which
+// log p of x = (x - m) - log l, lse = m + log l and entropy = log l - a / l.
+// Everything is taken about m, not about zero, so nothing large cancels, also
+// in rows that hold nothing but the type's lowest value. Elements that may be among the
 // row's top_k (bounded below by the threads' maxima, then by the top_k found so
 // far) go to a list in LDS and are ranked there by value, then by lowest index.
 // logprobs_join folds a row's splits.
@@ -27,6 +26,12 @@ constexpr int kCandidates = 1024;          // list of a chunk's candidates in LD
 constexpr int kJoinKeys = 2048;            // keys of all splits that the join holds in LDS
 constexpr int kJoinSplits = 64;            // a lane each
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+// Largest |m| whose elements take their distances by one fma: 4000 x 32000 bf16
+// in 47.3 us, by a subtraction and a product 49.6 (600 x 128256, 5 likeliest:
+// 51.6 and 55.5). Past it the rounding of m log2(e) would be more than 2^-17,
+// and near 2^31 more than exp2 takes.
+constexpr float kNear = 128.f;
 
 // The order of top_k on floats: the sign-magnitude order of their bits, so
 // that -0 < +0 and NaN (positive) is above +inf. 0 is below every float's
@@ -44,7 +49,6 @@ __device__ __forceinline__ uint64_t key_of(float x, int64_t i) {
   return ((uint64_t)order_of(x) << 32) | (uint32_t)~(uint32_t)i;
 }
 
-constexpr float kLn2 = 0.69314718055994530942f;
 
 // One thread's or split's softmax state.
 struct Soft {
@@ -53,7 +57,7 @@ struct Soft {
 // The state about the larger maximum m >= s.m.
 __device__ __forceinline__ void raise(Soft& s, float m) {
   // A side of no elements has l = a = 0 at -inf: its shift is made finite.
-  const float d = fmaxf(s.m - m, -1e4f), f = exp2f(d);
+  const float d = fmaxf(s.m - m, -1e4f), f = __builtin_amdgcn_exp2f(d * kLog2e);
   s.a = f * (s.a + d * s.l);
   s.l *= f;
   s.m = m;
@@ -115,18 +119,17 @@ struct Results {
   float *logprobs, *entropy, *lse, *top_logprobs;
   int32_t* top_tokens;
 };
-__device__ __forceinline__ float lse_of(const Soft& s) { return fmaf(s.m, kLn2, log2f(s.l) * kLn2); }
 // By one thread: the row's numbers, `chosen` its token's logit.
 __device__ __forceinline__ void write_row(const Results& r, int64_t row, const Soft& s, bool known, float chosen) {
-  const float lse = lse_of(s);
-  r.logprobs[row] = known ? chosen - lse : 0.f;
-  r.entropy[row] = (log2f(s.l) - s.a / s.l) * kLn2;
-  r.lse[row] = lse;
+  const float log_l = logf(s.l);
+  r.logprobs[row] = known ? (chosen - s.m) - log_l : 0.f;
+  r.entropy[row] = log_l - s.a / s.l;
+  r.lse[row] = s.m + log_l;
 }
 // By the workgroup: the row's likeliest tokens, ranked.
-__device__ __forceinline__ void write_top(const Results& r, int64_t row, float lse, const uint64_t* best, int top_k) {
+__device__ __forceinline__ void write_top(const Results& r, int64_t row, float m, float log_l, const uint64_t* best, int top_k) {
   for (int i = threadIdx.x; i < top_k; i += kThreads) {
-    r.top_logprobs[row * top_k + i] = value_of((uint32_t)(best[i] >> 32)) - lse;
+    r.top_logprobs[row * top_k + i] = (value_of((uint32_t)(best[i] >> 32)) - m) - log_l;
     r.top_tokens[row * top_k + i] = (int32_t)~(uint32_t)best[i];
   }
 }
@@ -174,19 +177,36 @@ __global__ void __launch_bounds__(kThreads)
       }
       if (tid == 0) count_s = 0;
     }
-    const float m = fmaxf(s.m, cm * kLog2e);
+    const float m = fmaxf(s.m, cm);
     if (m > s.m) raise(s, m);  // also the first finite chunk, from l = a = 0
     const float ref = m == -INFINITY ? 0.f : m;
+    // -inf weighs nothing: its distance is made finite for a's product.
+    if (fabsf(ref) <= kNear) {
+      // y = d log2(e) by one fma. What m log2(e) is rounded by is in all of
+      // them, a part in 2^24 of m, as lse's own rounding is.
+      const float ref2 = ref * kLog2e;
+      float a2 = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+      for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        // -inf weighs nothing: its distance is made finite for a's product.
-        const float y = __builtin_elementwise_maximum(fmaf((float)v[i][e], kLog2e, -ref), -1e4f);
-        const float w = __builtin_amdgcn_exp2f(y);
-        s.l += w;
-        s.a = fmaf(w, y, s.a);
-      }
+        for (int e = 0; e < E; ++e) {
+          const float y = __builtin_elementwise_maximum(fmaf((float)v[i][e], kLog2e, -ref2), -1e4f);
+          const float w = __builtin_amdgcn_exp2f(y);
+          s.l += w;
+          a2 = fmaf(w, y, a2);
+        }
+      s.a = fmaf(a2, kLn2, s.a);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float d = __builtin_elementwise_maximum((float)v[i][e] - ref, -1e4f);
+          const float w = __builtin_amdgcn_exp2f(d * kLog2e);
+          s.l += w;
+          s.a = fmaf(w, d, s.a);
+        }
+    }
     if constexpr (kTop) {
       const int64_t left = hi - base;
       __syncthreads();
@@ -262,7 +282,7 @@ __global__ void __launch_bounds__(kThreads)
       const bool known = token >= 0 && token < p.V;
       write_row(r, row, t, known, known ? (float)x[token] : 0.f);
     }
-    if constexpr (kTop) write_top(r, row, lse_of(t), best[turn], p.top_k);
+    if constexpr (kTop) write_top(r, row, t.m, logf(t.l), best[turn], p.top_k);
     return;
   }
   uint32_t* out = part + (row * nsplit + split) * split_words(p.top_k);
@@ -331,7 +351,7 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
   rank_keys(keys, count_s, best, 0, best, p.top_k);
   __syncthreads();
-  write_top(r, row, __shfl(lse_of(s), 0), best, p.top_k);
+  write_top(r, row, __shfl(s.m, 0), logf(__shfl(s.l, 0)), best, p.top_k);
 }
 
 // Elementwise over the logits, a row's numbers read once a workgroup.

@@ -320,7 +320,10 @@ __device__ __forceinline__ void any_part(const Shape& s, const Unit& u, const T*
           if (d < D) dot = fmaf(qv[j], (float)kr[d], dot);
           vv[j] = d < D ? (float)vr[d] : 0.f;
         }
-        const float x = wave_sum(dot) * s.p.scale * kLog2e;
+        float x = wave_sum(dot) * s.p.scale * kLog2e;
+        // Rounded here, not in a fma below: the largest is 0 off itself,
+        // however large.
+        asm("" : "+v"(x));
         if (l < 0.f) l = 0.f;
         const float mn = fmaxf(m, x);
         const float ref = mn == -INFINITY ? 0.f : mn;

@@ -217,6 +217,22 @@ def test_paged_attention_results_do_not_depend_on_the_pages_order(client):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("dim", [40, 64, 128, 500])
+def test_paged_attention_large_scores(client, dtype, dim):
+    """Two keys of one score far past the rest, and past what exp2 takes: each
+    weighs a half."""
+    rng = np.random.default_rng(3)
+    k, v = (put(x, dtype) for x in rng.standard_normal((2, 4, 1, 16, dim)))
+    k[:, :, :, :] = put(np.full((4, 1, 16, dim), -2.0 ** 18), dtype)
+    k[1, 0, 3], k[2, 0, 9] = (put(np.full(dim, 2.0 ** 17), dtype),) * 2
+    q = put(np.full((1, 2, dim), 2.0 ** 17), dtype)
+    table, n = np.array([[0, 1, 2, 3]], np.int32), np.array([60], np.int32)
+    (got,) = call(client, lambda b, p: b.paged_attention(*p, scale=1.0), [q, k, v, table, n], [dtype] * 3 + ["s32"] * 2)
+    want = (val(v)[1, 0, 3] + val(v)[2, 0, 9]) / 2
+    close(got, np.broadcast_to(want, (1, 2, dim)), (U[dtype] + 2 * W) * np.abs(want) + 2 * W * np.abs(val(v)[1, 0, 3]))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("size,dim", [(8, 64), (16, 128), (48, 64), (5, 96), (7, 40)])
 def test_paged_attention_full_tables_at_the_pools_end(client, dtype, size, dim):
     """Sequences that fill their table, the last page the pool's last, with
@@ -581,6 +597,35 @@ def test_token_logprobs_grad_is_the_forward_passs_difference(client):
             e = np.zeros_like(x)
             e[r, i] = s
             assert abs((loss(x + e) - loss(x - e)) / (2 * s) - dx[r, i]) < 10 * s * s
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("vocab,k", [(50, 3), (9000, 0), (20001, 12), (600000, 4)])
+def test_token_logprobs_large_logits(client, dtype, vocab, k):
+    """Rows of nothing but a mask's value, and logits at any size: the
+    distances to the largest count, not the logits' own size."""
+    rng = np.random.default_rng(9)
+    low = -3.38e38
+    x = np.stack([np.full(vocab, -1e30), np.full(vocab, low), np.full(vocab, -low), np.full(vocab, -1e9),
+                  1e9 + 64.0 * rng.integers(0, 3, vocab), np.where(np.arange(vocab) % 7, low, -low),
+                  np.where(np.arange(vocab) % 5, low, 3.0), 1000 + rng.standard_normal(vocab),
+                  -200 + rng.standard_normal(vocab), np.where(np.arange(vocab) == vocab - 1, 1e30, -5.0)])
+    x = put(x, dtype)
+    tok = rng.integers(0, vocab, len(x)).astype(np.int32)
+    got = call(client, lambda b, p: b.token_logprobs(*p, top_k=k), [x, tok], [dtype, "s32"])
+    want = P.token_logprobs(val(x), tok, k)
+    # Nothing but lse itself is off by a part of its size: the tolerances are
+    # those of the distances to the largest logit.
+    m = val(x).max(1, keepdims=True)
+    tol, ent_tol = logprob_tolerances(val(x) - m, np.log(np.exp(val(x) - m).sum(1)))
+    close(got[2], want[2], tol + 4 * W * np.abs(want[2]))
+    # Lowest less largest is -6.76e38, which rounds to -inf: past 2^128 - 2^103.
+    rounded = np.where(want[0] < -(2.0 ** 128 - 2.0 ** 103), -np.inf, want[0])
+    close(got[0], rounded, tol + 4 * W * np.abs(want[0]))
+    close(got[1], want[1], ent_tol)
+    if k:
+        assert np.array_equal(got[4], want[4])
+        close(got[3], want[3], tol[:, None] + 4 * W * np.abs(want[3]))
 
 
 # ---------------------------------------------------- the caller's addresses
