@@ -376,6 +376,8 @@ __global__ void __launch_bounds__(kThreads)
   const float g = known ? d_logprobs[row] : 0.f, h = d_entropy[row], z = lse[row], H = entropy[row];
   // h == 0 leaves the entropy out: where it is NaN or infinite, and g's part alone is not.
   const float c0 = h == 0.f ? -g : -fmaf(h, H, g);
+  // A row that no gradient reaches has none, whatever it holds (a padded row).
+  const bool none = g == 0.f && h == 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int64_t at = base + (int64_t)(i * kThreads + threadIdx.x) * E;
@@ -387,7 +389,7 @@ __global__ void __launch_bounds__(kThreads)
       // p log p is 0 at p = 0: -inf's distance is made finite.
       const float d = __builtin_elementwise_maximum((float)v[i][e] - z, -1e4f);
       const float w = __builtin_amdgcn_exp2f(d * kLog2e);
-      float y = w * fmaf(-h, d, c0);
+      float y = none ? 0.f : w * fmaf(-h, d, c0);
       if (at + e == token) y += g;
       o[e] = (T)y;
     }

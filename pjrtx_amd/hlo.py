@@ -439,7 +439,9 @@ class Builder:
 
     def token_logprobs_grad(self, logits: T, tokens: T, lse: T, entropy: T, d_logprobs: T, d_entropy: T) -> T:
         """The logits' gradient from those of token_logprobs' log probabilities
-        and entropies (f32 [N]), and the lse and entropy it gave."""
+        and entropies (f32 [N]), and the lse and entropy it gave. A row that
+        neither gradient reaches has zeros, whatever its logits are. The
+        probabilities are exp(logits - lse), as close as f32 holds lse."""
         return self.operator_call("pjrtx.token_logprobs_grad", [logits, tokens, lse, entropy, d_logprobs, d_entropy],
                                   [(logits.shape, logits.dtype)])[0]
 

@@ -578,6 +578,21 @@ def test_token_logprobs_grad(client, dtype, rows, vocab):
     close(got, want, 2 * W * (p * part * (8 + 4 * d) + hit) + U[dtype] * np.abs(want) + (6e-8 if dtype == "f16" else 1e-38))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_token_logprobs_grad_of_rows_left_out(client, dtype):
+    """Padded rows: no gradient reaches them, and none comes out, also where
+    they hold no distribution."""
+    x = np.ones((5, 9000))
+    x[0], x[1, 5], x[2, 7] = -np.inf, np.nan, np.inf
+    tok = np.array([3, -1, 9000, -1, 4], np.int32)
+    g, h = np.array([0, 5, -5, 7, 0], np.float32), np.zeros(5, np.float32)
+    with np.errstate(all="ignore"):
+        _, H, lse = (a.astype(np.float32) for a in P.token_logprobs(x, tok))
+    (dx,) = call(client, lambda b, p: b.token_logprobs_grad(*p), [put(x, dtype), tok, lse, H, g, h],
+                 [dtype, "s32"] + ["f32"] * 4)
+    assert np.isnan(lse[:3]).all() and (val(dx) == 0).all()
+
+
 def test_token_logprobs_grad_is_the_forward_passs_difference(client):
     rng = np.random.default_rng(11)
     x = rng.standard_normal((2, 30)).astype(np.float32)
