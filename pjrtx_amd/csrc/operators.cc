@@ -59,7 +59,8 @@ class Checker {
     const double v = std::strtod(it->second.c_str(), &end);
     // MLIR writes infinities and NaNs as hexadecimal bits.
     const bool bits = it->second.find_first_of("xX") < it->second.find(':');
-    need(end != it->second.c_str() && at_type(end) && !bits, std::string(key) + " must be a finite number");
+    need(end != it->second.c_str() && at_type(end) && !bits && std::isfinite(static_cast<float>(v)),
+         std::string(key) + " must be a finite number");
     return v;
   }
   int64_t integer(const char* key, int64_t dflt) const {
@@ -104,7 +105,6 @@ void lower_paged_attention(const Checker& c, Op* op) {
          "lengths must be s32 [batch]");
   c.need(c.out(0) == q, "the result must have q's shape and type");
   const double scale = c.number("scale", 1.0 / std::sqrt(static_cast<double>(q.dims[2])));
-  c.need(std::isfinite(scale), "scale must be finite");
   const int64_t window = c.integer("window", 0);
   c.need(window >= 0, "window must not be negative");
   c.within(q.dims[2] <= 512, "head dim above 512");
@@ -151,7 +151,7 @@ void check_rows(const Checker& c, const TensorType& x, const TensorType& gain) {
 
 double epsilon(const Checker& c) {
   const double eps = c.number("eps", 1e-5);
-  c.need(std::isfinite(eps) && eps >= 0, "eps must be finite and not negative");
+  c.need(eps >= 0, "eps must not be negative");
   return eps;
 }
 
@@ -246,7 +246,15 @@ bool lower_operator_call(const Program& prog, Op* op) {
   };
   auto it = targets.find(op->target);
   if (it == targets.end()) return false;
-  it->second(Checker(prog, *op), op);
+  const Checker c(prog, *op);
+  // The checks multiply dims in 64 bits.
+  for (const std::vector<int>* values : {&op->operands, &op->results})
+    for (int v : *values) {
+      int64_t n = 8;
+      for (int64_t d : prog.type(v).dims)
+        c.within(!__builtin_mul_overflow(n, std::max<int64_t>(d, 1), &n), "a tensor of 2^60 elements or more");
+    }
+  it->second(c, op);
   op->name = op->target;
   return true;
 }

@@ -160,7 +160,7 @@ def test_attributes_as_jax_prints_them(plugin):
     ins, outs = CALLS[ATT]
     text = text_of(ATT, ins, outs, {"scale": 0.25, "window": 7})
     assert len(plan(plugin, text)["steps"]) == 1
-    for value in ("0x7F800000 : f32", "0xFFC00000 : f32", "true", '"1.0"', "[1.0]", "1.0.0 : f32"):
+    for value in ("1.0e39 : f64", "-1.0e300 : f64", "0x7F800000 : f32", "0xFFC00000 : f32", "true", '"1.0"', "[1.0]", "1.0.0 : f32"):
         with pytest.raises(PjrtError) as e:
             plan(plugin, text.replace("2.50000000000000000e-01 : f64", value))
         assert e.value.code == INVALID and "scale" in e.value.message
@@ -184,3 +184,16 @@ def test_bytes_of_a_step_are_those_it_moves(plugin):
     assert step["algorithmic_bytes"] == 4 * 7 * 2 * 64 * 2 + 4 * 7
     step = plan(plugin, _append(False))["steps"][0]
     assert step["algorithmic_bytes"] == 4 * 7 * 2 * 64 * 2 + 4 * 7 + 4 * 8 * 2 * 16 * 64 * 2
+
+
+def test_refuses_shapes_whose_products_wrap(plugin):
+    """2^32 x 2^32 rows are no rows in 64 bits."""
+    big = ((2 ** 32, 2 ** 32, 8), "f32")
+    with pytest.raises(PjrtError) as e:
+        plan(plugin, text_of("pjrtx.add_rms_norm", [big, ((8,), "f32")], [big]))
+    assert e.value.code == UNIMPLEMENTED and "2^60" in e.value.message
+    pages = ((2 ** 32, 2 ** 32, 16, 64), "bf16")
+    ins, outs = CALLS[ATT]
+    with pytest.raises(PjrtError) as e:
+        plan(plugin, text_of(ATT, [pages if t[0] == PAGES else t for t in ins], outs))
+    assert e.value.code == UNIMPLEMENTED
