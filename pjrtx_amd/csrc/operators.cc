@@ -247,6 +247,7 @@ bool lower_operator_call(const Program& prog, Op* op) {
   auto it = targets.find(op->target);
   if (it == targets.end()) return false;
   const Checker c(prog, *op);
+  c.need(op->config.count("backend_config") == 0, "backend_config must be a dictionary");
   // The checks multiply dims in 64 bits.
   for (const std::vector<int>* values : {&op->operands, &op->results})
     for (int v : *values) {

@@ -1005,8 +1005,11 @@ void Parser::parse_generic_attrs(const std::string& dict, Op* op) {
     } else if (key == "call_target_name") {
       const size_t q0 = val.find('"'), q1 = val.rfind('"');
       if (q0 != std::string::npos && q1 > q0) op->target = val.substr(q0 + 1, q1 - q0 - 1);
-    } else if (key == "backend_config" && op->kind == OpKind::kCustomCall && val.size() >= 2 && val[0] == '{') {
-      op->config = split_attr_dict(val.substr(1, val.rfind('}') - 1));
+    } else if ((key == "backend_config" || key == "mhlo.backend_config") && op->kind == OpKind::kCustomCall) {
+      // A dictionary (JAX writes it under either name, beside an empty string);
+      // any other text is kept whole for the operators to refuse.
+      if (val.size() >= 2 && val[0] == '{') op->config = split_attr_dict(val.substr(1, val.rfind('}') - 1));
+      else if (val != "\"\"") op->config["backend_config"] = val;
     } else if (key == "dot_dimension_numbers") {
       size_t lt = val.find('<');
       size_t gt = val.rfind('>');

@@ -166,6 +166,16 @@ def test_attributes_as_jax_prints_them(plugin):
         assert e.value.code == INVALID and "scale" in e.value.message
     for value in ("9.99999974E-6 : f32", "1 : i64", "0.5", "-2.0e+00 : f64"):
         assert plan(plugin, text.replace("2.50000000000000000e-01 : f64", value))["steps"]
+    config = text[text.index("backend_config = {"):text.index("}", text.index("backend_config = {")) + 1]
+    assert "scale" in config and "window" in config
+    text = text.replace("window = 7", "window = -7")
+    for form in (config, 'backend_config = "", mhlo.' + config, "mhlo." + config + ', backend_config = ""'):
+        with pytest.raises(PjrtError) as e:
+            plan(plugin, text.replace(config.replace("= 7", "= -7"), form.replace("= 7", "= -7")))
+        assert "window" in e.value.message
+    with pytest.raises(PjrtError) as e:
+        plan(plugin, text.replace(config.replace("= 7", "= -7"), 'backend_config = "window=7"'))
+    assert e.value.code == INVALID and "dictionary" in e.value.message
     ins, outs = CALLS[APP]
     text = text_of(APP, ins, outs).replace(
         "backend_config = {}", "backend_config = {}, has_side_effect = false, operand_layouts = [dense<[3, 2, 1, 0]> : "
