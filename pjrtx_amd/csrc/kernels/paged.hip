@@ -16,6 +16,15 @@
 //
 // A share of a row that is not all of it writes its softmax's (max, sum,
 // unnormalised output) to scratch; paged_combine folds them in order.
+//
+// Long caches are bound by HBM: 2 sequences of 131072 keys by 8 heads of 128,
+// f16, 537 MB in 99 us (5.4 TB/s), the 64 ragged ones 538 MB in 101 us. The
+// fold takes 4 us where few keys do (600 keys: 5.6 + 4.3 us, all of it the
+// latency of dependent reads: length, table, keys) and 8 at those sizes, about
+// half of it behind the tiles. In the last arriving workgroup instead of its
+// own launch it was no faster (10.7 and 10.5 us at 600 keys; 17.4 and 13.9 at
+// 7 x 1500 f32), and a device-scope fence for it cost the tiles their L2 (321
+// us for 101).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
