@@ -36,9 +36,9 @@ constexpr int64_t kMaxIndex = (int64_t(1) << 31) - 1;
 bool is_operator_float(DType t) { return t == DType::kF32 || t == DType::kF16 || t == DType::kBF16; }
 bool is_index(DType t) { return t == DType::kS32 || t == DType::kS64; }
 
-class Checker {
+class CallArgs {
  public:
-  Checker(const Program& prog, const Op& op) : prog_(prog), op_(op) {}
+  CallArgs(const Program& prog, const Op& op) : prog_(prog), op_(op) {}
   const TensorType& in(size_t i) const { return prog_.type(op_.operands.at(i)); }
   const TensorType& out(size_t i) const { return prog_.type(op_.results.at(i)); }
   size_t ins() const { return op_.operands.size(); }
@@ -82,7 +82,7 @@ class Checker {
   const Op& op_;
 };
 
-void check_pages(const Checker& c, const TensorType& k, const TensorType& v) {
+void check_pages(const CallArgs& c, const TensorType& k, const TensorType& v) {
   c.need(k.rank() == 4 && k.dims == v.dims && k.dtype == v.dtype,
          "k_pages and v_pages must be [pages, kv_heads, page_size, head_dim] of one shape and type");
   c.need(is_operator_float(k.dtype), "pages must be f32, f16 or bf16");
@@ -91,7 +91,7 @@ void check_pages(const Checker& c, const TensorType& k, const TensorType& v) {
            "more than 2^31 - 1 rows of a head in the pages");
 }
 
-void lower_paged_attention(const Checker& c, Op* op) {
+void lower_paged_attention(const CallArgs& c, Op* op) {
   c.need(c.ins() == 5 && c.outs() == 1, "takes q, k_pages, v_pages, page_table and lengths, and has one result");
   c.known_keys({"scale", "window"});
   const TensorType &q = c.in(0), &k = c.in(1), &table = c.in(3), &lengths = c.in(4);
@@ -120,7 +120,7 @@ void lower_paged_attention(const Checker& c, Op* op) {
   op->oper.window = window;
 }
 
-void lower_paged_append(const Checker& c, Op* op) {
+void lower_paged_append(const CallArgs& c, Op* op) {
   c.need(c.ins() == 5 && c.outs() == 2, "takes k_pages, v_pages, k_new, v_new and slots, and has two results");
   c.known_keys({});
   const TensorType &k = c.in(0), &kn = c.in(2), &slots = c.in(4);
@@ -140,7 +140,7 @@ void lower_paged_append(const Checker& c, Op* op) {
 // Leading dims of x as rows.
 Dims rows_of(const TensorType& x) { return Dims(x.dims.begin(), x.dims.end() - 1); }
 
-void check_rows(const Checker& c, const TensorType& x, const TensorType& gain) {
+void check_rows(const CallArgs& c, const TensorType& x, const TensorType& gain) {
   c.need(is_operator_float(x.dtype), "the rows must be f32, f16 or bf16");
   c.need(x.rank() >= 1 && x.dims.back() > 0, "the rows must be [..., dim] with a dim of at least 1");
   c.need(gain.rank() == 1 && gain.dims[0] == x.dims.back() && gain.dtype == x.dtype,
@@ -149,13 +149,13 @@ void check_rows(const Checker& c, const TensorType& x, const TensorType& gain) {
   c.within(x.dims.back() <= (int64_t(1) << 28), "rows of more than 2^28 elements");
 }
 
-double epsilon(const Checker& c) {
+double epsilon(const CallArgs& c) {
   const double eps = c.number("eps", 1e-5);
   c.need(eps >= 0, "eps must not be negative");
   return eps;
 }
 
-void lower_add_rms_norm(const Checker& c, Op* op) {
+void lower_add_rms_norm(const CallArgs& c, Op* op) {
   c.need(c.ins() == 2 || c.ins() == 3, "takes x, a residual or none, and gain");
   c.known_keys({"eps"});
   const TensorType& x = c.in(0);
@@ -177,7 +177,7 @@ void lower_add_rms_norm(const Checker& c, Op* op) {
   op->oper.eps = epsilon(c);
 }
 
-void lower_add_rms_norm_grad(const Checker& c, Op* op) {
+void lower_add_rms_norm_grad(const CallArgs& c, Op* op) {
   c.need((c.ins() == 3 || c.ins() == 4) && c.outs() == 2,
          "takes dy, dsum or none, the sum and gain, and has two results");
   c.known_keys({"eps"});
@@ -191,7 +191,7 @@ void lower_add_rms_norm_grad(const Checker& c, Op* op) {
   op->oper.eps = epsilon(c);
 }
 
-void check_logits(const Checker& c) {
+void check_logits(const CallArgs& c) {
   const TensorType &x = c.in(0), &tokens = c.in(1);
   c.need(x.rank() == 2 && is_operator_float(x.dtype) && x.dims[1] > 0,
          "logits must be f32, f16 or bf16 [rows, vocabulary]");
@@ -201,7 +201,7 @@ void check_logits(const Checker& c) {
   c.within(x.dims[0] <= kMaxGroups && x.dims[0] * ((x.dims[1] + 8191) / 8192) <= kMaxGroups, "too many logits");
 }
 
-void lower_token_logprobs(const Checker& c, Op* op) {
+void lower_token_logprobs(const CallArgs& c, Op* op) {
   c.need(c.ins() == 2 && (c.outs() == 3 || c.outs() == 5),
          "takes logits and tokens, and has logprobs, entropy and lse, or these with top_logprobs and top_tokens");
   c.known_keys({});
@@ -221,7 +221,7 @@ void lower_token_logprobs(const Checker& c, Op* op) {
   op->kind = OpKind::kTokenLogprobs;
 }
 
-void lower_token_logprobs_grad(const Checker& c, Op* op) {
+void lower_token_logprobs_grad(const CallArgs& c, Op* op) {
   c.need(c.ins() == 6 && c.outs() == 1,
          "takes logits, tokens, lse, entropy, d_logprobs and d_entropy, and has one result");
   c.known_keys({});
@@ -235,7 +235,7 @@ void lower_token_logprobs_grad(const Checker& c, Op* op) {
 }  // namespace
 
 bool lower_operator_call(const Program& prog, Op* op) {
-  using Lower = void (*)(const Checker&, Op*);
+  using Lower = void (*)(const CallArgs&, Op*);
   static const std::map<std::string, Lower> targets = {
       {"pjrtx.paged_attention", lower_paged_attention},
       {"pjrtx.paged_append", lower_paged_append},
@@ -246,7 +246,7 @@ bool lower_operator_call(const Program& prog, Op* op) {
   };
   auto it = targets.find(op->target);
   if (it == targets.end()) return false;
-  const Checker c(prog, *op);
+  const CallArgs c(prog, *op);
   c.need(op->config.count("backend_config") == 0, "backend_config must be a dictionary");
   // The checks multiply dims in 64 bits.
   for (const std::vector<int>* values : {&op->operands, &op->results})
