@@ -13,9 +13,10 @@
 //
 // Many rows are bound by HBM (1000 x 32000 f32, 128 MB, in 26.7 us), or by the
 // exponentials beside it (4000 x 32000 bf16, 256 MB, in 47). Few rows are bound
-// by latency: 64 x 128256 bf16 with 20 likeliest 12.6 us in 8 splits a row, two
-// dependent chunks each with its maximum, bound, list and ranking, and 4.6 for
-// the join.
+// by latency: 64 x 128256 bf16 with 20 likeliest 12.1 us in 8 splits a row, two
+// dependent chunks each with its maximum, bound, list and ranking, and 4.2 for
+// the join. (Ranking only when the list is long saves barriers, but the looser
+// bound scans more: 4000 x 32000 bf16, 5 likeliest, 82 us for 72.)
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -103,18 +104,30 @@ __device__ __forceinline__ uint32_t wave_kth_u(uint32_t x, int k) {
 }
 
 // Ranks the n distinct keys at `cand` together with the `held` at `best` and
-// leaves the top_k largest in order at `to`. Called by the whole workgroup.
-__device__ __forceinline__ void rank_keys(const uint64_t* cand, int n, const uint64_t* best, int held, uint64_t* to,
-                                          int top_k) {
-  for (int i = threadIdx.x; i < n + held; i += kThreads) {
-    const uint64_t mine = i < n ? cand[i] : best[i - n];
+// leaves the top_k largest in order at `to`; kLanes lanes take a key. Called by
+// the whole workgroup.
+template <int kLanes>
+__device__ __forceinline__ void rank_keys_by(const uint64_t* cand, int n, const uint64_t* best, int held, uint64_t* to,
+                                             int top_k) {
+  const int lane = threadIdx.x % kLanes;
+  for (int i0 = 0; i0 < n + held; i0 += kThreads / kLanes) {
+    const int i = i0 + threadIdx.x / kLanes;
+    const uint64_t mine = i < n ? cand[i] : i < n + held ? best[i - n] : ~0ull;
     int above = 0;
 #pragma unroll 8
-    for (int j = 0; j < n; ++j) above += cand[j] > mine ? 1 : 0;
+    for (int j = lane; j < n; j += kLanes) above += cand[j] > mine ? 1 : 0;
 #pragma unroll 4
-    for (int j = 0; j < held; ++j) above += best[j] > mine ? 1 : 0;
-    if (above < top_k) to[above] = mine;
+    for (int j = lane; j < held; j += kLanes) above += best[j] > mine ? 1 : 0;
+#pragma unroll
+    for (int d = 1; d < kLanes; d <<= 1) above += __shfl_xor(above, d);
+    if (i < n + held && lane == 0 && above < top_k) to[above] = mine;
   }
+}
+__device__ __forceinline__ void rank_keys(const uint64_t* cand, int n, const uint64_t* best, int held, uint64_t* to,
+                                          int top_k) {
+  if (n + held <= kThreads / 4) rank_keys_by<4>(cand, n, best, held, to, top_k);
+  else if (n + held <= kThreads / 2) rank_keys_by<2>(cand, n, best, held, to, top_k);
+  else rank_keys_by<1>(cand, n, best, held, to, top_k);
 }
 
 __device__ __forceinline__ int64_t read_token(const void* tokens, int bytes, int64_t i) {
@@ -141,9 +154,10 @@ __device__ __forceinline__ void write_top(const Results& r, int64_t row, float m
 }
 
 // A workgroup's share of a row: elements [lo, hi). A row of one share is
-// finished here.
+// finished here. (5 waves a SIMD: 4000 x 32000 bf16, 5 likeliest, 70 us, with
+// the registers of 4 80.)
 template <typename T, bool kTop, bool kStream>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kTop ? 5 : 8)
     logprobs_split(LogprobsParams p, int nsplit, int64_t per, const T* __restrict__ logits,
                    const void* __restrict__ tokens, uint32_t* __restrict__ part, Results r) {
   constexpr int E = kVecElems<T>;
@@ -404,26 +418,32 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// Splits of a row, whole chunks each: those of the least estimated time, in the
-// 5 us that 4 workgroups on each CU take for a chunk. Many workgroups: a chunk
-// each costs 0.45 more to begin and end, and the last round is half empty. Few:
-// the time of one alone, 1.8 and 0.25 a chunk. The join: 0.45 and 0.05 a split.
-// (bf16, 20 likeliest, 64 x 128256: 16 splits a row 10.8 + 6.9 us, 8 splits 11.7
-// + 5.1; 600 x 128256, 5 likeliest: 16 splits 65 + 5 us, 1 split 53.)
+// Splits of a row, whole chunks each: those of the least estimated time, in us.
+// A workgroup alone takes `alone`; together they take `all`, of which the chip
+// does 1024 chunks, 4 workgroups a CU, in `unit` (by HBM for f32, by the
+// exponentials and the candidates for 16 bits), with 0.7 of a chunk to begin
+// and end each and half a round more where there are rounds; where both count,
+// they add as squares do. Measured (estimated), bf16, 20 likeliest, V = 128256:
+// 8 rows in 16 / 8 / 4 splits 12.4 / 13.9 / 19.6 us (13.1 / 14.4 / 18.6), 64 rows
+// in 16 / 8 17.6 / 16.2 (16.9 / 16.4), 128 rows in 8 / 4 / 2 20.7 / 22.8 / 28.7
+// (21.1 / 22.7 / 30.3); 5 likeliest: 256 rows in 4 / 2 / 1 26.8 / 31.6 / 38.1
+// (30.2 / 33.2 / 41.2), 256 rows of 32000 in 4 / 1 14.2 / 13.2 (14.3 / 13.5).
 struct Split {
   int n;
   int64_t per;
 };
-Split split_of(const LogprobsParams& p) {
+Split split_of(const LogprobsParams& p, DType t) {
   const int64_t chunks = (p.V + kChunk - 1) / kChunk;
   const int64_t most = std::min<int64_t>(chunks, p.top_k ? std::min(kJoinSplits, kJoinKeys / p.top_k) : kJoinSplits);
+  const double k = p.top_k, unit = t == DType::kF32 ? 6.5 : p.top_k ? 5.0 : 3.3;
   int64_t best = chunks;
   double least = INFINITY;
   for (int64_t n = 1; n <= most; ++n) {
     const int64_t per = (chunks + n - 1) / n;
-    const double rounds = static_cast<double>(p.rows) * n / 1024, group = per + 0.45;
-    const double time = std::max(rounds * group + (rounds > 1 ? 0.5 * group : 0), 1.8 + 0.25 * per) +
-                        (n > 1 ? 0.45 + 0.05 * n : 0);
+    const double rounds = static_cast<double>(p.rows) * n / 1024;
+    const double all = unit * (per + 0.7) * (rounds > 1 ? rounds + 0.5 : rounds);
+    const double alone = p.top_k ? 4.3 + 0.025 * k + (1.8 + 0.03 * k) * per : 3.4 + 1.5 * per;
+    const double time = std::sqrt(all * all + alone * alone) + (n == 1 ? 0 : p.top_k ? 3.6 + 0.007 * n * k : 3.2);
     if (time < least) {
       least = time;
       best = per;
@@ -440,7 +460,7 @@ void check_launch(const char* what) {
 }  // namespace
 
 size_t token_logprobs_scratch_bytes(const LogprobsParams& p, DType t) {
-  const int n = split_of(p).n;
+  const int n = split_of(p, t).n;
   return n > 1 ? static_cast<size_t>(p.rows) * n * split_words(p.top_k) * sizeof(uint32_t) : 0;
 }
 
@@ -448,7 +468,7 @@ void launch_token_logprobs(hipStream_t s, const LogprobsParams& p, DType t, cons
                            float* logprobs, float* entropy, float* lse, float* top_logprobs, int32_t* top_tokens,
                            void* scratch) {
   if (p.rows == 0) return;
-  const Split sp = split_of(p);
+  const Split sp = split_of(p, t);
   const dim3 grid(static_cast<uint32_t>(p.rows * sp.n)), block(kThreads);
   uint32_t* part = static_cast<uint32_t*>(scratch);
   const Results r = {logprobs, entropy, lse, top_logprobs, top_tokens};
