@@ -216,12 +216,12 @@ class PagedRunner:
         self.token = np.zeros(cfg.batch, np.int32)
 
     def _hold(self, place: int, keys: int) -> None:
-        """Pages for `keys` keys of the sequence at `place`."""
-        for i in range(-(-keys // self.cfg.page_size)):
-            if self.table[place, i] < 0:
-                if not self.free:
-                    raise MemoryError("no free page")
-                self.table[place, i] = self.free.pop()
+        """Pages for `keys` keys of the sequence at `place`, or none."""
+        need = [i for i in range(-(-keys // self.cfg.page_size)) if self.table[place, i] < 0]
+        if len(need) > len(self.free):
+            raise MemoryError("no free page")
+        for i in need:
+            self.table[place, i] = self.free.pop()
 
     def _run(self, exe, args):
         outs = exe.execute_buffers(self.weights + [self.client.buffer(a) for a in args] + self.pools)
@@ -233,8 +233,9 @@ class PagedRunner:
         generated token, its logits, and the prompt's scores: the log
         probability of each token but the first after those before it."""
         n = len(prompt)
-        if not 1 <= n <= self.cfg.chunk:
-            raise ValueError(f"a prompt has 1 to {self.cfg.chunk} tokens")
+        most = min(self.cfg.chunk, self.cfg.model.max_len)
+        if not 1 <= n <= most:
+            raise ValueError(f"a prompt has 1 to {most} tokens")
         places = np.flatnonzero(self.length < 0)
         if not len(places):
             raise ValueError("no empty place")

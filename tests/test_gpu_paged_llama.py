@@ -161,6 +161,29 @@ def test_a_captured_step_replays_like_an_eager_one(client, run_fresh):
     assert run.decode.graph_stats()["replays"] > 0
 
 
+def test_prompts_that_find_no_room_take_nothing(client):
+    cfg = dataclasses.replace(CFG, pages=3, chunk=64)
+    run = G.PagedRunner(client, cfg, weights(cfg)[0])
+    run.add(np.arange(16, dtype=np.int32))
+    with pytest.raises(MemoryError):
+        run.add(np.arange(9, dtype=np.int32))
+    with pytest.raises(ValueError, match="1 to 40"):
+        run.add(np.zeros(41, np.int32))
+    assert len(run.free) == 1 and (run.table[1:] < 0).all() and (run.length >= 0).sum() == 1
+    run.step()
+    assert not run.free
+    run.leave(0)
+    assert sorted(run.free) == [0, 1, 2]
+
+
+def test_a_loss_of_no_rows_is_zero(client):
+    rng = np.random.default_rng(6)
+    args = [ops.f32_to_bf16_bits(rng.standard_normal(s).astype(np.float32)) for s in ((5, 64), (5, 64), (64,), (64, 100))]
+    tok = np.array([-1, 100, -7, 2 ** 31 - 1, -2 ** 31], np.int32)
+    loss, *grads = client.compile(programs.lm_head_loss(5, 64, 100, 0.1))(*args, tok, dtypes=["bf16"] * 4 + [None])
+    assert loss == 0 and all((ops.bf16_bits_to_f32(g) == 0).all() for g in grads)
+
+
 @pytest.mark.parametrize("rows,d,vocab,weight", [(1, 64, 100, 0.0), (7, 96, 333, 0.1), (130, 128, 1000, 0.0)])
 def test_loss_and_gradients(client, rows, d, vocab, weight):
     """Each result against float64 on the same inputs. The bf16 roundings on
