@@ -36,8 +36,8 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 // Largest |m| whose elements take their distances by one fma: 4000 x 32000 bf16
 // in 47.3 us, by a subtraction and a product 49.6 (600 x 128256, 5 likeliest:
-// 51.6 and 55.5). Past it the rounding of m log2(e) would be more than 2^-17,
-// and near 2^31 more than exp2 takes.
+// 51.6 and 55.5). Past it the rounding of m log2(e), which the chunk's sums are
+// corrected by, would be more than 2^-17, and near 2^31 more than exp2 takes.
 constexpr float kNear = 128.f;
 
 // The order of top_k on floats: the sign-magnitude order of their bits, so
@@ -202,20 +202,25 @@ __global__ void __launch_bounds__(kThreads, kTop ? 5 : 8)
     const float ref = m == -INFINITY ? 0.f : m;
     // -inf weighs nothing: its distance is made finite for a's product.
     if (fabsf(ref) <= kNear) {
-      // y = d log2(e) by one fma. What m log2(e) is rounded by is in all of
-      // them, a part in 2^24 of m, as lse's own rounding is.
-      const float ref2 = ref * kLog2e;
-      float a2 = 0.f;
+      // y = d log2(e) + r by one fma, r what rounding m log2(e) left (a fma
+      // gives it exactly). The chunk's sums give it back: over 2^r = 1 + c, |c|
+      // below 2^-17, to c^2. The largest element's 1 + c becomes 1, so that no
+      // sum is below 1 and no log probability above 0.
+      const float ref2 = ref * kLog2e, r = fmaf(ref, kLog2e, -ref2);
+      float l2 = 0.f, a2 = 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           const float y = __builtin_elementwise_maximum(fmaf((float)v[i][e], kLog2e, -ref2), -1e4f);
           const float w = __builtin_amdgcn_exp2f(y);
-          s.l += w;
+          l2 += w;
           a2 = fmaf(w, y, a2);
         }
-      s.a = fmaf(a2, kLn2, s.a);
+      const float c = __builtin_amdgcn_exp2f(r) - 1.f;
+      a2 = fmaf(-r, l2, a2);
+      s.l += fmaf(-c, l2, l2);
+      s.a = fmaf(fmaf(-c, a2, a2), kLn2, s.a);
     } else {
 #pragma unroll
       for (int i = 0; i < NV; ++i)

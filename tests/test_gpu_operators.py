@@ -643,6 +643,35 @@ def test_token_logprobs_large_logits(client, dtype, vocab, k):
         close(got[3], want[3], tol[:, None] + 4 * W * np.abs(want[3]))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("vocab,k,step", [(300, 4, 0.5), (9000, 0, 6.5), (40000, 0, 8.5), (40000, 4, 8.5)])
+@pytest.mark.parametrize("equal", [1, 3])
+def test_token_logprobs_wherever_the_largest_logit_lies(client, dtype, vocab, k, step, equal):
+    """Rows with all their weight on `equal` tokens, at a largest logit of any
+    size: log p is -log(equal) whatever that size is. The other weights are
+    e^-110, below every float, so a sum of one weight over itself is 1 and log
+    p is 0; of three it is off by their 3 roundings, the quotient's and the
+    logarithm's 4 w of itself."""
+    rng = np.random.default_rng(vocab)
+    top = np.arange(-128, 128.5, step)
+    x = np.repeat(top[:, None] - 110, vocab, 1)
+    at = np.stack([rng.permutation(vocab)[:equal] for _ in top])
+    at[::2] = (at[::2, :1] // 4 * 4 + np.arange(equal)) % vocab  # neighbours: one thread's
+    np.put_along_axis(x, at, top[:, None], 1)
+    x = put(x, dtype)
+    assert np.array_equal(val(x).max(1), top)
+    tok = at[:, -1].astype(np.int32)
+    got = call(client, lambda b, p: b.token_logprobs(*p, top_k=k), [x, tok], [dtype, "s32"])
+    want = np.log(equal)
+    tol = 0 if equal == 1 else 2 * (4 + 4 * want) * W
+    assert (np.abs(got[0] + want) <= tol).all(), np.abs(got[0] + want).max()
+    assert (got[0] <= 0).all() and (np.abs(got[1] - want) <= tol + W).all()
+    assert (np.abs(got[2] - (top + want)) <= tol + W * np.abs(top + want)).all()
+    if k:
+        assert (np.abs(got[3][:, :equal] + want) <= tol).all()
+        assert np.array_equal(got[4][:, :equal], np.sort(at, 1))
+
+
 # ---------------------------------------------------- the caller's addresses
 
 def _off(client, a, by):
