@@ -234,27 +234,27 @@ def test_paged_attention_large_scores(client, dtype, dim):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
-@pytest.mark.parametrize("group", [1, 20])
-def test_paged_attention_many_small_weights(client, dtype, group):
-    """One key of weight 1 and value 0 before 40,000 of weight e^-18, below f16's
-    smallest number, and value 1: together they weigh 6e-4."""
-    n, size, dim = 40000, 64, 64
-    pages = -(-n // size)
-    k, v = np.zeros((2, pages, 1, size, dim))
-    k[..., 0] = -18
-    v[...] = 1
-    k[0, 0, 0, 0] = v[0, 0, 0] = 0
-    q = np.zeros((1, group, dim))
-    q[..., 0] = 1
-    table = np.arange(pages, dtype=np.int32)[None]
-    (got,) = call(client, lambda b, p: b.paged_attention(*p, scale=1.0),
-                  [put(q, dtype), put(k, dtype), put(v, dtype), table, np.array([n], np.int32)], [dtype] * 3 + ["s32"] * 2)
-    s = (n - 1) * np.exp(-18.0)
-    want = np.full((1, group, dim), s / (1 + s))
-    # sums of n weights in 32 bits, each off by its exponent's 26 w and 4 w, and
-    # by u squared; the result's rounding, in f16 below its normal numbers
+@pytest.mark.parametrize("kv_heads,group,dim,size", [(2, 4, 64, 16), (1, 20, 128, 8), (2, 1, 256, 16), (1, 3, 96, 24), (2, 2, 80, 16)])
+def test_paged_attention_weights_are_not_rounded_to_the_type(client, dtype, kv_heads, group, dim, size):
+    """Scores that are exact: small integers times a power of two. A weight is
+    then off by its exponent's rounding (two of |x| w), its exponential's 4 w
+    and, in 16 bits, by the square of the type's u, what two pieces of it leave;
+    the sums by (n + 8) w. All of it counts by the weight's own share of the
+    answer, in the numerator and in the denominator."""
+    rng = np.random.default_rng(dim)
+    lengths = [1, 3, 9, 33, 80, 500]
+    k, v, table = cache(rng, lengths, kv_heads, size, dim, dtype, poison=False)
+    k = put(rng.integers(-2, 3, k.shape), dtype)
+    q = put(rng.integers(-2, 3, (len(lengths), kv_heads * group, dim)), dtype)
+    scale = 2.0 ** -4
+    (got,) = call(client, lambda b, p: b.paged_attention(*p, scale=scale), [q, k, v, table, np.array(lengths, np.int32)],
+                  [dtype] * 3 + ["s32"] * 2)
+    want = P.paged_attention(val(q), val(k), val(v), table, lengths, scale)
+    share = P.paged_attention(val(q), val(k), np.abs(val(v)), table, lengths, scale)  # sum of p |v|
+    x = 1.45 * scale * 4 * dim
     u2 = 0 if dtype == "f32" else U[dtype] ** 2
-    close(got, want, 2 * ((n + 40) * W + u2) * want + U[dtype] * want + (2.0 ** -25 if dtype == "f16" else 0))
+    weight = u2 + (2 * x + 4 + np.array(lengths)[:, None, None] + 8) * W
+    close(got, want, 2 * weight * 2 * share + U[dtype] * np.abs(want))
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
