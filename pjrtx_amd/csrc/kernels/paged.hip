@@ -426,6 +426,12 @@ __device__ __forceinline__ float groups_max(float x) {
   return fmaxf(__builtin_bit_cast(float, (uint32_t)w[0]), __builtin_bit_cast(float, (uint32_t)w[1]));
 }
 
+// What a weight of 1 goes to the matrix steps as, and counts as in its sum. f16
+// holds 2^-24 at least and 65504 at most: as 2^14 a weight loses at most 2^-39
+// there, and 2^20 of them 2^-19; as 1 they would lose 2^-5.
+template <typename T>
+constexpr float kLift = std::is_same_v<T, f16_t> ? 16384.f : 1.f;
+
 // N dwords at p, which is aligned to an element only.
 template <int N>
 __device__ __forceinline__ void load_words(const void* p, uint32_t* w) {
@@ -584,7 +590,7 @@ __device__ __forceinline__ void use_tile(float scale2, Tile<T, D>& t, Heads<T, D
 #pragma unroll
   for (int h = 0; h < Sh::kHalves; ++h)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x[h][r] = __builtin_amdgcn_exp2f(x[h][r] - ref);
+    for (int r = 0; r < 4; ++r) x[h][r] = __builtin_amdgcn_exp2f(x[h][r] - ref) * kLift<T>;
   if constexpr (Sh::kHalf) {
     // A weight goes to the matrix steps in two pieces of the type, what the
     // first leaves in the second: to the square of the type's rounding. They are

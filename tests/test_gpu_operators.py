@@ -257,6 +257,30 @@ def test_paged_attention_weights_are_not_rounded_to_the_type(client, dtype, kv_h
     close(got, want, 2 * weight * 2 * share + U[dtype] * np.abs(want))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("group", [1, 20])
+def test_paged_attention_many_small_weights(client, dtype, group):
+    """One key of weight 1 and value 0 before 7,999 of weight e^-18, which is
+    below f16's smallest number, and value 100. Sequences enough that one
+    workgroup walks each: all of one page table."""
+    n, size, dim, batch = 8000, 64, 64, 600
+    pages = n // size
+    k, v = np.zeros((2, pages, 1, size, dim))
+    k[..., 0], v[...] = -18, 100
+    k[0, 0, 0, 0] = v[0, 0, 0] = 0
+    q = np.zeros((batch, group, dim))
+    q[..., 0] = 1
+    table = np.repeat(np.arange(pages, dtype=np.int32)[None], batch, 0)
+    (got,) = call(client, lambda b, p: b.paged_attention(*p, scale=1.0),
+                  [put(q, dtype), put(k, dtype), put(v, dtype), table, np.full(batch, n, np.int32)], [dtype] * 3 + ["s32"] * 2)
+    s = (n - 1) * np.exp(-18.0)
+    want = np.full((batch, group, dim), 100 * s / (1 + s))
+    # sums of n weights in 32 bits, each off by its exponent's 2 x 26 w, its
+    # exponential's 4 w and by u squared; the result's rounding
+    u2 = 0 if dtype == "f32" else U[dtype] ** 2
+    close(got, want, (2 * ((n + 56) * W + u2) + U[dtype]) * want)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("size,dim", [(8, 64), (16, 128), (48, 64), (5, 96), (7, 40)])
 def test_paged_attention_full_tables_at_the_pools_end(client, dtype, size, dim):
