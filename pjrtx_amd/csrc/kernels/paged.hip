@@ -432,21 +432,6 @@ __device__ __forceinline__ float groups_max(float x) {
 template <typename T>
 constexpr float kLift = std::is_same_v<T, f16_t> ? 16384.f : 1.f;
 
-// N dwords at p, which is aligned to an element only.
-template <int N>
-__device__ __forceinline__ void load_words(const void* p, uint32_t* w) {
-  typedef uint32_t words __attribute__((ext_vector_type(N < 2 ? 2 : N)));
-  typedef words unaligned __attribute__((aligned(2)));
-  typedef uint32_t one __attribute__((aligned(2)));
-  if constexpr (N == 1) {
-    w[0] = *static_cast<const one*>(p);
-  } else {
-    const words v = *static_cast<const unaligned*>(p);
-#pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = v[i];
-  }
-}
-
 template <typename T, int D>
 struct TileShape {
   static constexpr bool kHalf = sizeof(T) == 2;

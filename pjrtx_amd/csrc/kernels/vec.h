@@ -54,6 +54,26 @@ __device__ __forceinline__ void store_vec(T* p, int64_t n, const typename Vec<T>
     if (e < n) p[e] = v[e];
 }
 
+// N dwords at p, which is aligned to an element only, and not a byte past them:
+// a vector of 3 may be read as one of 4, and the last row's ends the memory.
+template <int N>
+__host__ __device__ __forceinline__ void load_words(const void* p, uint32_t* w) {
+  typedef uint32_t one __attribute__((aligned(2)));
+  if constexpr (N == 1) {
+    w[0] = *static_cast<const one*>(p);
+  } else if constexpr (N == 3) {
+    load_words<2>(p, w);
+    load_words<1>(static_cast<const one*>(p) + 2, w + 2);
+  } else {
+    typedef uint32_t words __attribute__((ext_vector_type(N)));
+    typedef words unaligned __attribute__((aligned(2)));
+    static_assert(sizeof(words) == 4 * N, "as many bytes as words");
+    const words v = *static_cast<const unaligned*>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = v[i];
+  }
+}
+
 __device__ __forceinline__ float wave_sum(float x) {
 #pragma unroll
   for (int k = 32; k >= 1; k >>= 1) x += __shfl_xor(x, k);
