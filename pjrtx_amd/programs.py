@@ -133,16 +133,20 @@ def lm_head_loss(rows: int, d_model: int, vocab: int, entropy_weight: float = 0.
     """The end of a decoder's training step and its gradients: h, t =
     add_rms_norm(x, residual, gain); logits = h.W; loss = the mean over rows
     whose target is in the vocabulary of -log p(target), less entropy_weight of
-    the entropy (0, with gradients of 0, where no row's is). Returns (loss, d x = d residual, d gain, d W), everything but
-    the loss bf16."""
+    the entropy (0, with gradients of 0, where no row's is). The other rows
+    count as zeros whatever they hold. Returns (loss, d x = d residual, d gain,
+    d W), everything but the loss bf16."""
     b = Builder("jit_lm_head_loss")
     x, residual = b.param((rows, d_model), "bf16"), b.param((rows, d_model), "bf16")
     gain, w, targets = b.param((d_model,), "bf16"), b.param((d_model, vocab), "bf16"), b.param((rows,), "s32")
+    known = b.and_(b.compare("GE", targets, b.scalar_like(0, targets)),
+                   b.compare("LT", targets, b.scalar_like(vocab, targets)))
+    held = b.broadcast_in_dim(known, x.shape, [0])
+    x, residual = (b.select(held, a, b.scalar_like(0.0, a)) for a in (x, residual))
     h, t = b.add_rms_norm(x, residual, gain, eps)
     logits = b.dot_general(h, w, contract=((1,), (0,)))
     lp, entropy, lse = b.token_logprobs(logits, targets)
-    live = b.convert(b.and_(b.compare("GE", targets, b.scalar_like(0, targets)),
-                            b.compare("LT", targets, b.scalar_like(vocab, targets))), "f32")
+    live = b.convert(known, "f32")
     count = b.sum(live, [0])
     share = b.divide(live, b.broadcast_in_dim(b.maximum(count, b.scalar_like(1.0, count)), live.shape, []))
     gained = b.add(lp, b.multiply(entropy, b.scalar_like(entropy_weight, entropy)))

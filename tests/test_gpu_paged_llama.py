@@ -184,6 +184,30 @@ def test_a_loss_of_no_rows_is_zero(client):
     assert loss == 0 and all((ops.bf16_bits_to_f32(g) == 0).all() for g in grads)
 
 
+@pytest.mark.parametrize("weight", [0.0, 0.1])
+def test_rows_left_out_of_the_loss_may_hold_anything(client, weight):
+    """Rows without a target, of NaN, infinities and numbers beyond bf16: the
+    loss and the gradients are those of the same rows at zero, and their own
+    gradient is zero."""
+    rng = np.random.default_rng(8)
+    bf = lambda a: ops.f32_to_bf16_bits(np.asarray(a, np.float32))  # noqa: E731
+    x, res = rng.standard_normal((2, 9, 64))
+    g, w = bf(1 + 0.1 * rng.standard_normal(64)), bf(rng.standard_normal((64, 100)) * 0.125)
+    tok = rng.integers(0, 100, 9).astype(np.int32)
+    out = [1, 4, 6, 8]
+    tok[out] = [-1, 100, -1, -5]
+    exe = client.compile(programs.lm_head_loss(9, 64, 100, weight))
+    x[out] = res[out] = 0
+    want = exe(bf(x), bf(res), g, w, tok, dtypes=["bf16"] * 4 + [None])
+    x[1, 3], x[4], res[6], x[8] = np.nan, np.inf, -np.inf, 3e38
+    res[8] = 3e38
+    got = exe(bf(x), bf(res), g, w, tok, dtypes=["bf16"] * 4 + [None])
+    assert np.isfinite(want[0])
+    for a, b in zip(got, want):
+        assert a.tobytes() == b.tobytes()
+    assert (ops.bf16_bits_to_f32(got[1][out]) == 0).all()
+
+
 @pytest.mark.parametrize("rows,d,vocab,weight", [(1, 64, 100, 0.0), (7, 96, 333, 0.1), (130, 128, 1000, 0.0)])
 def test_loss_and_gradients(client, rows, d, vocab, weight):
     """Each result against float64 on the same inputs. The bf16 roundings on
