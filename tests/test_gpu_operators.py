@@ -8,6 +8,8 @@ is off by, plus 4 w for the exponential; where the weights are rounded to 16
 bits before the product with the values, by u more, in the sum and in the
 product. Each bound is written where it is used, doubled for the rounding of
 the bound's own terms."""
+import time
+
 import numpy as np
 import pytest
 
@@ -378,6 +380,45 @@ def test_append_allocation_free_writes_the_callers_pages(client):
     assert np.array_equal(read(args[1]), wk) and np.array_equal(read(args[0]), wv)
     for d in args + outs:
         d.free()
+
+
+def test_append_time_grows_as_its_rows_do(client):
+    """2^20 rows are 16 times 2^16 of them, and the search for later rows of a
+    slot no more: the square of 16 would be 256. Best of several, in one
+    process, against the shorter call."""
+    def best(n):
+        b = Builder()
+        pages, shape = (n // 64, 1, 64, 8), (n, 1, 8)
+        p = [b.param(pages, "bf16", donate=True) for _ in range(2)] + [b.param(shape, "bf16") for _ in range(2)]
+        exe = client.compile(b.build(list(b.paged_append(*p, b.param((n,), "s32")))))
+        d = [DeviceArray(client.p, 16 * n) for _ in range(4)]
+        d.append(DeviceArray.from_numpy(client.p, np.random.default_rng(n).permutation(n).astype(np.int32)))
+        times = []
+        for _ in range(6):
+            client.p.hip_check(client.p.lib.pjrtx_hip_synchronize(0))
+            t = time.perf_counter()
+            exe.execute_noalloc([a.ptr for a in d], [d[0].ptr, d[1].ptr])
+            client.p.hip_check(client.p.lib.pjrtx_hip_synchronize(0))
+            times.append(time.perf_counter() - t)
+        for a in d:
+            a.free()
+        return min(times)
+    short, long = best(1 << 16), best(1 << 20)
+    assert long <= 48 * short, (short, long)
+
+
+@pytest.mark.parametrize("n", [8192, 8193, 50000])
+def test_append_many_rows_of_equal_slots(client, n):
+    """The last of the rows of a slot stays, however far apart they lie."""
+    rng = np.random.default_rng(n)
+    pages = (40, 2, 8, 4)
+    k, v = (put(x, "bf16") for x in rng.standard_normal((2, *pages)))
+    kn, vn = (put(x, "bf16") for x in rng.standard_normal((2, n, 2, 4)))
+    slots = rng.integers(-3, 40 * 8 + 3, n).astype(np.int64)
+    slots[n // 2:] = np.where(slots[n // 2:] % 2 == 0, -1, slots[n // 2:])  # even ones only in the first half
+    got = call(client, lambda b, p: b.paged_append(*p), [k, v, kn, vn, slots], ["bf16"] * 4 + ["s64"])
+    for g, w in zip(got, P.paged_append(k, v, kn, vn, slots)):
+        assert np.array_equal(g, w)
 
 
 # -------------------------------------------------------------------- norm
