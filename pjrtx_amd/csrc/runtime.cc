@@ -564,6 +564,52 @@ Executable::Executable(Program prog, Plan plan, std::string fingerprint, std::st
     w->trips = s.while_trips;
     loops_[si] = std::move(w);
   }
+  plan_noalloc();
+}
+
+void Executable::plan_noalloc() {
+  NoallocPlan& n = noalloc_;
+  for (int v : prog_.params) n.param_bytes.push_back(prog_.type(v).bytes());
+  for (int v : prog_.results) n.result_bytes.push_back(prog_.type(v).bytes());
+  std::map<int, int64_t> result_of;  // -1: more than one
+  for (size_t i = 0; i < prog_.results.size(); ++i) {
+    const auto [it, fresh] = result_of.emplace(prog_.results[i], static_cast<int64_t>(i));
+    if (!fresh) it->second = -1;
+  }
+  // Values that are a written parameter's buffer: the parameter's position.
+  std::map<int, int> buffer_of;
+  for (int k : plan_.written_params) buffer_of[prog_.params[k]] = k;
+  auto same_buffer = [&](int from, int to) {
+    const auto it = buffer_of.find(from);
+    if (it != buffer_of.end()) buffer_of[to] = it->second;
+  };
+  for (const Step& st : plan_.steps) {
+    if (st.kind == StepKind::kAlias) same_buffer(st.inputs[0], st.outputs[0]);
+    for (const auto& [pos, ww] : st.window_out) same_buffer(ww.operand, st.outputs[pos]);
+    bool oper = false;
+    if (st.kind == StepKind::kLibrary) {
+      const Op& op = prog_.ops[st.lib_op];
+      oper = operator_lib_kind(op.kind) != LibKind::kCopy;
+      if (st.in_place) same_buffer(op.operands[0], st.outputs[0]);
+      for (size_t i = 0; st.in_place_operands >> i; ++i)
+        if (st.in_place_operands >> i & 1) same_buffer(op.operands[i], st.outputs[i]);
+    }
+    if (!oper && st.kind != StepKind::kLoop) continue;
+    for (size_t i = 0; i < st.outputs.size(); ++i) {
+      const auto it = result_of.find(st.outputs[i]);
+      if (it == result_of.end() || it->second < 0) continue;
+      if (st.window_out.count(static_cast<int>(i)) || (i < 32 && (st.in_place_operands >> i & 1))) continue;
+      n.places.push_back({st.outputs[i], static_cast<size_t>(it->second), oper});
+    }
+  }
+  for (int k : plan_.written_params) {
+    const int64_t to = prog_.param_alias.at(k);
+    const bool keeps = to >= 0 && to < static_cast<int64_t>(prog_.results.size()) &&
+                       prog_.type(prog_.results[to]) == prog_.type(prog_.params[k]) &&
+                       buffer_of.count(prog_.results[to]) && buffer_of[prog_.results[to]] == k;
+    n.kept_result.push_back(keeps ? to : -1);
+    n.keeps = n.keeps || keeps;
+  }
 }
 
 int64_t Executable::while_trips(size_t si) const {
@@ -1167,58 +1213,58 @@ size_t Executable::execute_noalloc(Device* dev, const void* const* args, size_t 
     m->borrowed = true;
     vals[prog_.params[i]] = m;
   }
-  // Results that go straight to the caller's memory.
-  auto overlaps = [](const void* a, size_t na, const void* b, size_t nb) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return na && nb && x < y + nb && y < x + na;
-  };
-  auto alone = [&](size_t i, int param) {  // output i against all arguments (but `param`) and other outputs
-    const size_t n = prog_.type(prog_.results[i]).bytes();
-    for (size_t k = 0; k < num_args; ++k)
-      if (static_cast<int>(k) != param && overlaps(outs[i], n, args[k], prog_.type(prog_.params[k]).bytes())) return false;
-    for (size_t k = 0; k < num_outs; ++k)
-      if (k != i && overlaps(outs[i], n, outs[k], prog_.type(prog_.results[k]).bytes())) return false;
-    return n > 0;
-  };
-  // Whether `result` is parameter k's buffer after the plan's in-place writes.
-  auto keeps_buffer = [&](int k, int result) {
-    std::set<int> held = {prog_.params[k]};
-    for (const Step& st : plan_.steps) {
-      if (st.kind == StepKind::kAlias && held.count(st.inputs[0])) held.insert(st.outputs[0]);
-      for (const auto& [pos, ww] : st.window_out)
-        if (held.count(ww.operand)) held.insert(st.outputs[pos]);
-      if (st.kind != StepKind::kLibrary) continue;
-      const Op& op = prog_.ops[st.lib_op];
-      if (st.in_place && held.count(op.operands[0])) held.insert(st.outputs[0]);
-      for (size_t i = 0; st.in_place_operands >> i; ++i)
-        if ((st.in_place_operands >> i & 1) && held.count(op.operands[i])) held.insert(st.outputs[i]);
+  // Which results go straight to the caller's memory: those whose output
+  // overlaps nothing else of the call, an argument that keeps its buffer aside.
+  std::vector<MemRef> placed;
+  std::vector<bool> kept(plan_.written_params.size(), false);
+  if (!noalloc_.places.empty() || noalloc_.keeps) {
+    std::vector<char> own(num_args, 0);  // arguments that their result is given back at
+    for (size_t w = 0; w < kept.size(); ++w) {
+      const int64_t to = noalloc_.kept_result[w];
+      kept[w] = to >= 0 && outs[to] == args[plan_.written_params[w]];
+      if (kept[w]) own[plan_.written_params[w]] = 1;
     }
-    return held.count(result) > 0;
-  };
-  std::vector<MemRef> placed(prog_.values.size());
-  for (const Step& st : plan_.steps) {
-    const bool oper = st.kind == StepKind::kLibrary && operator_lib_kind(prog_.ops[st.lib_op].kind) != LibKind::kCopy;
-    if (!oper && st.kind != StepKind::kLoop) continue;
-    for (int v : st.outputs) {
-      const auto first = std::find(prog_.results.begin(), prog_.results.end(), v);
-      if (first == prog_.results.end() || std::count(first, prog_.results.end(), v) > 1) continue;
-      const size_t i = first - prog_.results.begin();
-      // The generated kernels' vector stores take blocks as the arena's.
-      if (!alone(i, -1) || (!oper && reinterpret_cast<uintptr_t>(outs[i]) % 256 != 0)) continue;
+    struct Span {
+      uintptr_t lo, hi;
+      int64_t out;  // -1: an argument
+    };
+    std::vector<Span> spans;
+    spans.reserve(num_args + num_outs);
+    auto add = [&](const void* p, size_t n, int64_t out) {
+      const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
+      if (n) spans.push_back({lo, lo + n, out});
+    };
+    for (size_t i = 0; i < num_args; ++i)
+      if (!own[i]) add(args[i], noalloc_.param_bytes[i], -1);
+    for (size_t i = 0; i < num_outs; ++i) add(outs[i], noalloc_.result_bytes[i], static_cast<int64_t>(i));
+    std::sort(spans.begin(), spans.end(), [](const Span& x, const Span& y) { return x.lo < y.lo; });
+    // In order of their starts, every span that meets another meets the one
+    // that reaches furthest before it, or is that one.
+    std::vector<char> alone(num_outs, 0);
+    for (const Span& x : spans)
+      if (x.out >= 0) alone[x.out] = 1;
+    const Span* far = nullptr;
+    for (const Span& x : spans) {
+      if (far && x.lo < far->hi)
+        for (const Span* y : {&x, far})
+          if (y->out >= 0) alone[y->out] = 0;
+      if (!far || x.hi > far->hi) far = &x;
+    }
+    for (size_t w = 0; w < kept.size(); ++w) kept[w] = kept[w] && alone[noalloc_.kept_result[w]];
+    for (const NoallocPlan::Place& pl : noalloc_.places) {
+      if (!alone[pl.result] || (!pl.any_address && reinterpret_cast<uintptr_t>(outs[pl.result]) % 256 != 0)) continue;
+      if (placed.empty()) placed.resize(prog_.values.size());
       auto m = std::make_shared<DeviceMemory>();
       m->dev = dev;
-      m->ptr = outs[i];
-      m->bytes = m->capacity = prog_.type(v).bytes();
+      m->ptr = outs[pl.result];
+      m->bytes = m->capacity = noalloc_.result_bytes[pl.result];
       m->borrowed = true;
-      placed[v] = m;
+      placed[pl.value] = m;
     }
   }
-  for (int k : plan_.written_params) {
-    const int64_t to = prog_.param_alias.at(k);
-    if (to >= 0 && to < static_cast<int64_t>(num_outs) && outs[to] == args[k] &&
-        prog_.type(prog_.results[to]) == prog_.type(prog_.params[k]) && alone(to, k) &&
-        keeps_buffer(k, prog_.results[to]))
-      continue;  // given back in the same memory: written where it is
+  for (size_t w = 0; w < kept.size(); ++w) {
+    if (kept[w]) continue;  // given back in the same memory: written where it is
+    const int k = plan_.written_params[w];
     // The plan writes this parameter in place: work on a copy, the caller's
     // input stays as it was.
     const MemRef& src = vals[prog_.params[k]];
@@ -1230,7 +1276,7 @@ size_t Executable::execute_noalloc(Device* dev, const void* const* args, size_t 
   }
   for (auto& [v, m] : L->constants) vals[v] = m;
   for (size_t si = 0; si < plan_.steps.size(); ++si) {
-    run_step(L, si, vals, -1, &placed);
+    run_step(L, si, vals, -1, placed.empty() ? nullptr : &placed);
     for (int v : plan_.steps[si].release_after) vals[v].reset();
   }
   for (size_t i = 0; i < num_outs; ++i) {

@@ -365,8 +365,23 @@ class Executable {
   };
   void run_while(Loaded* L, size_t si, std::vector<MemRef>& vals);
 
+  // What the allocation-free execute needs of the plan besides its steps.
+  struct NoallocPlan {
+    struct Place {
+      int value;         // a result that a step can write where the caller wants it,
+      size_t result;     // its position,
+      bool any_address;  // and whether the step takes any element's address
+    };
+    std::vector<Place> places;
+    std::vector<int64_t> kept_result;  // per written parameter: the result that is its buffer, or -1
+    bool keeps = false;                // any of these
+    std::vector<size_t> param_bytes, result_bytes;
+  };
+  void plan_noalloc();
+
   Program prog_;
   Plan plan_;
+  NoallocPlan noalloc_;
   std::map<size_t, std::unique_ptr<WhileLoop>> loops_;
   std::string fingerprint_, name_;
   std::vector<char> code_;
