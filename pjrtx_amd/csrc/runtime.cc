@@ -576,6 +576,8 @@ void Executable::plan_noalloc() {
     const auto [it, fresh] = result_of.emplace(prog_.results[i], static_cast<int64_t>(i));
     if (!fresh) it->second = -1;
   }
+  std::set<int> read;
+  for (const Step& st : plan_.steps) read.insert(st.inputs.begin(), st.inputs.end());
   // Values that are a written parameter's buffer: the parameter's position.
   std::map<int, int> buffer_of;
   for (int k : plan_.written_params) buffer_of[prog_.params[k]] = k;
@@ -595,11 +597,12 @@ void Executable::plan_noalloc() {
         if (st.in_place_operands >> i & 1) same_buffer(op.operands[i], st.outputs[i]);
     }
     if (!oper && st.kind != StepKind::kLoop) continue;
+    // Other kernels take a value as the blocks they know lie.
     for (size_t i = 0; i < st.outputs.size(); ++i) {
       const auto it = result_of.find(st.outputs[i]);
       if (it == result_of.end() || it->second < 0) continue;
       if (st.window_out.count(static_cast<int>(i)) || (i < 32 && (st.in_place_operands >> i & 1))) continue;
-      n.places.push_back({st.outputs[i], static_cast<size_t>(it->second), oper});
+      n.places.push_back({st.outputs[i], static_cast<size_t>(it->second), oper && !read.count(st.outputs[i])});
     }
   }
   for (int k : plan_.written_params) {

@@ -314,7 +314,8 @@ class Executable {
   // block comes from the device's fixed no-allocation block (kernels/
   // noalloc.h), whose contents the previous call left behind. A result that
   // an operator or a generated elementwise kernel produces is written straight
-  // to its output (elementwise: at a multiple of 256 bytes), and an
+  // to its output (at a multiple of 256 bytes, but for operators' results that no
+  // other step reads), and an
   // output at the address of the donated argument that the plan writes in
   // place for it (the argument's `tf.aliasing_output`) is written there, where
   // no other argument or output of the call overlaps either. Work is queued
@@ -370,7 +371,7 @@ class Executable {
     struct Place {
       int value;         // a result that a step can write where the caller wants it,
       size_t result;     // its position,
-      bool any_address;  // and whether the step takes any element's address
+      bool any_address;  // and whether it may lie at any element's address
     };
     std::vector<Place> places;
     std::vector<int64_t> kept_result;  // per written parameter: the result that is its buffer, or -1

@@ -813,6 +813,31 @@ def test_addresses_are_an_elements(client, dtype, what):
             d.free()
 
 
+@pytest.mark.parametrize("by", [2, 6, 16, 256])
+def test_results_that_other_steps_read(client, by):
+    """A norm of keys that is a result, at any address, and attention's operand,
+    whose kernels load whole vectors: the bits of aligned ones."""
+    rng = np.random.default_rng(14)
+    x, q, v = (put(rng.standard_normal((1, 256, 4, 128)), "bf16") for _ in range(3))
+    g, zero = put(np.ones(128), "bf16"), np.array(0, np.int32)
+    b = Builder()
+    ps = [b.param(x.shape, "bf16") for _ in range(3)] + [b.param((128,), "bf16"), b.param((), "s32")]
+    (k,) = b.add_rms_norm(ps[0], None, ps[3])
+    o = b.custom_call("pjrtx.mlx_metal.scaled_dot_product_attention", [ps[1], k, ps[2], ps[4]], x.shape, "bf16")
+    w = b.dot_general(b.reshape(k, (1024, 128)), b.reshape(ps[1], (1024, 128)), contract=((0,), (0,)))
+    exe = client.compile(b.build([k, o, w]))
+    want = exe(x, q, v, g, zero, dtypes=["bf16"] * 4 + [None])
+    ins = [DeviceArray.from_numpy(client.p, a) for a in (x, q, v, g, zero)]
+    outs = [DeviceArray(client.p, a.nbytes + by) for a in want]
+    for _ in range(2):
+        exe.execute_noalloc([d.ptr for d in ins], [d.ptr + by for d in outs])
+        client.p.hip_check(client.p.lib.pjrtx_hip_synchronize(0))
+        for d, a in zip(outs, want):
+            assert np.array_equal(d.to_numpy(np.uint8, (a.nbytes + by,))[by:], a.view(np.uint8).ravel())
+    for d in ins + outs:
+        d.free()
+
+
 # ------------------------------------------------------------ inside a loop
 
 def test_append_and_attention_inside_a_while_loop(client):
