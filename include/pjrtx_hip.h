@@ -163,13 +163,16 @@ PJRTX_HIP_API int pjrtx_executable_run_pjrt(struct PJRT_LoadedExecutable* exe, s
  * then holds the result; every other argument is left as it was. Outputs must
  * not overlap each other, nor arguments but in that way, for a kernel to write
  * them itself; where they do, the result is copied there at the end.
+ * Outputs, and caches written at their own address, are written while the plan
+ * runs: a call that fails may have written any part of them.
  * Every intermediate value, every copy of a parameter the plan writes in
  * place, and every kernel scratch
  * block (split-reduction partials, split-K partials, sort keys, scatter
  * segments) is carved from one fixed device block per GPU of
  * pjrtx_noalloc_scratch_bytes() bytes (64 MiB), held from the first call on
  * that GPU until the process ends. A program whose needs exceed it fails with
- * PJRT_Error_Code_RESOURCE_EXHAUSTED (outputs then unspecified); programs with
+ * PJRT_Error_Code_RESOURCE_EXHAUSTED (outputs and such caches then unspecified,
+ * as steps before the one that found no room have run); programs with
  * a while loop fail with UNIMPLEMENTED. The call calls no hipMalloc or
  * hipFree and no allocating library routine; the work is queued on the
  * device's stream and the call returns without waiting
