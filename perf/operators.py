@@ -226,13 +226,9 @@ _EPS = 1e-5
 _client = None
 
 
-def _compiled(c, inputs):
-    """The program that makes the case's call, loaded."""
-    global _client
+def _program(c, inputs):
+    """The program that makes the case's call."""
     from pjrtx_amd.hlo import Builder
-    from pjrtx_amd.pjrt import Client
-    if _client is None:
-        _client = Client()
     names = {v: k for k, v in _TORCH.items()}
     kind = c["kind"]
     b = Builder("jit_" + kind)
@@ -243,9 +239,12 @@ def _compiled(c, inputs):
         out = list(b.paged_append(*p))
     elif kind == "norm" and c["quantize"]:
         # The next operator's view of the 8-bit rows: the values they stand for.
-        y, scale, total = b.add_rms_norm(*p, eps=_EPS, quantize=True)
-        y = b.multiply(b.convert(y, "f32"), b.broadcast_in_dim(scale, y.shape, [0]))
-        out = [b.convert(y, c["dtype"]), scale, total]
+        # The rows themselves are a result too, in the caller's memory: as a value
+        # between the two steps they could be more than the 64 MiB that such a
+        # call has for all of them.
+        y8, scale, total = b.add_rms_norm(*p, eps=_EPS, quantize=True)
+        y = b.multiply(b.convert(y8, "f32"), b.broadcast_in_dim(scale, y8.shape, [0]))
+        out = [b.convert(y, c["dtype"]), scale, total, y8]
     elif kind == "norm":
         out = list(b.add_rms_norm(*p, eps=_EPS))
     elif kind == "norm_grad":
@@ -254,7 +253,16 @@ def _compiled(c, inputs):
         out = list(b.token_logprobs(*p, top_k=c["top_k"]))
     else:
         out = [b.token_logprobs_grad(*p)]
-    return _client.compile(b.build(out))
+    return b.build(out)
+
+
+def _compiled(c, inputs):
+    """That program, loaded."""
+    global _client
+    from pjrtx_amd.pjrt import Client
+    if _client is None:
+        _client = Client()
+    return _client.compile(_program(c, inputs))
 
 
 def prepare(case, seed):
@@ -267,7 +275,11 @@ def prepare(case, seed):
         state["out"] = inputs[:2] if case["kind"] == "append" else [
             torch.empty(shape, dtype=_TORCH[t], device="cuda") for shape, t in _results(case)]
         state["in_ptrs"] = [x.data_ptr() for x in inputs]
-        state["out_ptrs"] = [x.data_ptr() for x in state["out"]]
+        held = []
+        if case["kind"] == "norm" and case["quantize"]:
+            held = [torch.empty((case["rows"], case["dim"]), dtype=torch.int8, device="cuda")]
+        state["held"] = held
+        state["out_ptrs"] = [x.data_ptr() for x in state["out"] + held]
     return state
 
 
