@@ -1,6 +1,8 @@
 """Lowering, refusals and plans of the operator custom calls (no GPU)."""
 import json
+import re
 
+import numpy as np
 import pytest
 
 from pjrtx_amd.hlo import Builder
@@ -207,3 +209,34 @@ def test_refuses_shapes_whose_products_wrap(plugin):
     with pytest.raises(PjrtError) as e:
         plan(plugin, text_of(ATT, [pages if t[0] == PAGES else t for t in ins], outs))
     assert e.value.code == UNIMPLEMENTED
+
+
+def test_performance_cases_leave_room_in_the_fixed_block(plugin):
+    """What a case's program holds between its steps, besides results, which lie
+    in the caller's memory: within the allocation-free call's block, at the
+    largest rows of 8 bits that a draw's bound lets pass too."""
+    import random
+
+    import torch
+
+    from perf import operators as cases
+
+    room = plugin.lib.pjrtx_noalloc_scratch_bytes()
+    size = {"bf16": 2, "f16": 2, "f32": 4, "i8": 1, "i32": 4}
+    rng = random.Random(5)
+    most = [{"kind": "norm", "rows": r, "dim": d, "quantize": True, "dtype": t}
+            for r, d, t in ((8200, 8192, "bf16"), (8192, 8256, "f16"), (16384, 4160, "bf16"), (4192, 16384, "f16"))]
+    most = [c for c in most if cases.work(c)["bytes"] <= cases._MOST and cases._held(c) <= 4 * cases._MOST]
+    assert len(most) == 4
+    for c in most + [c for c in cases.listed() if c["kind"] == "norm"] + [cases.draw(rng) for _ in range(300)]:
+        if c["kind"] != "norm":
+            continue
+        x = torch.empty((c["rows"], c["dim"]), dtype=cases._TORCH[c["dtype"]], device="meta")
+        text = cases._program(c, [x, x, x[0]])
+        line = next(s for s in text.splitlines() if s.strip().startswith(("return ", "func.return ", "stablehlo.return ")))
+        results = 0
+        for t in re.findall(r"tensor<([^>]*)>", line):
+            *dims, name = t.split("x")
+            results += size[name] * int(np.prod([int(d) for d in dims]))
+        held = sum(n for s in plan(plugin, text)["steps"] for n in s["out_bytes"]) - results
+        assert 0 <= held <= room, (c, held)
