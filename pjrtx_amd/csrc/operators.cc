@@ -105,6 +105,8 @@ void lower_paged_attention(const CallArgs& c, Op* op) {
          "lengths must be s32 [batch]");
   c.need(c.out(0) == q, "the result must have q's shape and type");
   const double scale = c.number("scale", 1.0 / std::sqrt(static_cast<double>(q.dims[2])));
+  // the kernels take scores in powers of two
+  c.need(std::isfinite(static_cast<float>(scale) * 1.44269504f), "scale times log2(e) must be a finite number");
   const int64_t window = c.integer("window", 0);
   c.need(window >= 0, "window must not be negative");
   c.within(q.dims[2] <= 512, "head dim above 512");

@@ -240,3 +240,14 @@ def test_performance_cases_leave_room_in_the_fixed_block(plugin):
             results += size[name] * int(np.prod([int(d) for d in dims]))
         held = sum(n for s in plan(plugin, text)["steps"] for n in s["out_bytes"]) - results
         assert 0 <= held <= room, (c, held)
+
+
+def test_refuses_a_scale_whose_scores_are_no_floats(plugin):
+    """Scores are taken times log2(e): 3e38 of that is beyond f32, and a score
+    of 0 would not be 0."""
+    ins, outs = CALLS[ATT]
+    for scale in (3e38, -2.5e38):
+        with pytest.raises(PjrtError) as e:
+            plan(plugin, text_of(ATT, ins, outs, {"scale": scale}))
+        assert e.value.code == INVALID and "scale" in e.value.message
+    assert plan(plugin, text_of(ATT, ins, outs, {"scale": 2.0 ** 127}))["steps"]
