@@ -11,12 +11,12 @@
 // far) go to a list in LDS and are ranked there by value, then by lowest index.
 // logprobs_join folds a row's splits.
 //
-// Many rows are bound by HBM (1000 x 32000 f32, 128 MB, in 26.7 us), or by the
-// exponentials beside it (4000 x 32000 bf16, 256 MB, in 47). Few rows are bound
-// by latency: 64 x 128256 bf16 with 20 likeliest 12.1 us in 8 splits a row, two
-// dependent chunks each with its maximum, bound, list and ranking, and 4.2 for
+// Many rows are bound by HBM (1000 x 32000 f32, 128 MB, in 26.9 us), or by the
+// exponentials beside it (4000 x 32000 bf16, 256 MB, in 48). Few rows are bound
+// by latency: 64 x 128256 bf16 with 20 likeliest 11.5 us in 8 splits a row, two
+// dependent chunks each with its maximum, bound, list and ranking, and 4.1 for
 // the join. (Ranking only when the list is long saves barriers, but the looser
-// bound scans more: 4000 x 32000 bf16, 5 likeliest, 82 us for 72.)
+// bound scans more: 4000 x 32000 bf16, 5 likeliest, 14% longer.)
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -35,8 +35,8 @@ constexpr int kJoinSplits = 64;            // a lane each
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 // Largest |m| whose elements take their distances by one fma: 4000 x 32000 bf16
-// in 47.3 us, by a subtraction and a product 49.6 (600 x 128256, 5 likeliest:
-// 51.6 and 55.5). Past it the rounding of m log2(e), which the chunk's sums are
+// in 48.9 us, by a subtraction and a product 49.9 (600 x 128256, 5 likeliest:
+// 52.6 and 54.7). Past it the rounding of m log2(e), which the chunk's sums are
 // corrected by, would be more than 2^-17, and near 2^31 more than exp2 takes.
 constexpr float kNear = 128.f;
 
@@ -154,8 +154,8 @@ __device__ __forceinline__ void write_top(const Results& r, int64_t row, float m
 }
 
 // A workgroup's share of a row: elements [lo, hi). A row of one share is
-// finished here. (5 waves a SIMD: 4000 x 32000 bf16, 5 likeliest, 70 us, with
-// the registers of 4 80.)
+// finished here. (5 waves a SIMD: 4000 x 32000 bf16, 5 likeliest, 65 us, with
+// the registers of 4 72.)
 template <typename T, bool kTop, bool kStream>
 __global__ void __launch_bounds__(kThreads, kTop ? 5 : 8)
     logprobs_split(LogprobsParams p, int nsplit, int64_t per, const T* __restrict__ logits,

@@ -361,9 +361,12 @@ __global__ void __launch_bounds__(256)
 // Rows that the kernel above holds, this one and the next, without spilling: 2
 // vectors a thread of 512 (16 bits) or 1024 (f32).
 bool grad_in_registers(const NormParams& p) { return p.D <= 8192; }
-// Shares of dgain: two workgroups of 256 threads, or one of more, a CU. Rows and
-// the shares' sum, with two and with one of more: 4000 x 8192 bf16 56.7 + 6.8
+// Shares of dgain: two workgroups of up to 256 threads, or one of more, a CU. Rows
+// and the shares' sum, with two and with one of more: 4000 x 8192 bf16 56.7 + 6.8
 // and 51.3 + 5.0 us, 1283 x 4928 and 1000 x 8192 f32 33.5 + 6.5 and 27.8 + 4.8.
+// Rows of up to 64 vectors have one wave a workgroup, two a CU, and are bound by
+// its latency: 16384 x 512 bf16 31.0 + 4.7 us, 67 MB. Rows of more than 8192
+// elements are read twice: 1000 x 16384 bf16 23.3 + 59.5 + 11.8 us, 131 MB.
 int64_t grad_shares(const NormParams& p, DType t) {
   const int64_t nvec = (p.D + 16 / static_cast<int64_t>(dtype_size(t)) - 1) / (16 / static_cast<int64_t>(dtype_size(t)));
   return std::min<int64_t>(p.rows, nvec <= 512 || !grad_in_registers(p) ? 512 : 256);

@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(kWaves * 64)
 // columns then lie in the order lane, element, which the output undoes. No
 // LDS and no barrier until the waves' states meet.
 //
-// Bound by HBM: the matrix steps are 5% of a tile's time at 5 TB/s, whether a
+// Bound by HBM: the matrix steps are 8% of a tile's time at 5 TB/s, whether a
 // row has 1 head or 16. The next tile's rows are loaded before this one's are
 // used; head dims above 128 have no registers for that.
 
@@ -802,7 +802,7 @@ Shape shape_of(const PagedParams& p) {
   s.p = p;
   s.group = p.Hq / p.Hkv;
   // 8 sequences of 8192 keys, 8 heads of 128 with 32 query heads each, bf16:
-  // 90 us in rows of 16, 74 in rows of 32.
+  // 90 us in rows of 16, 73 in rows of 32, whose two sets load a tile each.
   s.sets = s.group <= kHeads || !takes_tiles(p.D) ? 1 : s.group <= 2 * kHeads ? 2 : kSets;
   s.sets_log = s.sets / 2;
   s.heads = std::min(s.group, kHeads * s.sets);
