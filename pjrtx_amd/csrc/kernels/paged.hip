@@ -399,20 +399,24 @@ __device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f3
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
                                                    0);
 }
+// Two weights in two pieces of the type, a first one below the weight and the rest
+// of it: 2^-16 of a weight is lost in bf16, 2^-21 in f16. No rest of a weight is
+// 0, so that an infinite value's product with it is no NaN: bf16 has room for a
+// least one, f16 leaves a part in 2^11 to it (a weight below 2^-28 of the largest
+// may have a rest of 0 all the same).
 template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (std::is_same_v<T, f16_t>)
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
-  else
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
-}
-
-template <typename T>
-__device__ __forceinline__ f32x2 unpack2(uint32_t w) {
-  if constexpr (std::is_same_v<T, f16_t>)
-    return __builtin_convertvector(__builtin_bit_cast(f16x2, w), f32x2);
-  else
-    return __builtin_convertvector(__builtin_bit_cast(bf16x2, w), f32x2);
+__device__ __forceinline__ void split2(float a, float b, uint32_t& first, uint32_t& rest) {
+  if constexpr (std::is_same_v<T, f16_t>) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(a * (1.f - 0x1p-11f), b * (1.f - 0x1p-11f));
+    first = __builtin_bit_cast(uint32_t, h);
+    rest = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a - (float)h[0], b - (float)h[1]}, f16x2));
+  } else {
+    const uint32_t u = __builtin_bit_cast(uint32_t, a), v = __builtin_bit_cast(uint32_t, b);
+    first = __builtin_amdgcn_perm(v, u, 0x07060302u);
+    const f32x2 r = {__builtin_amdgcn_fmed3f(a - __builtin_bit_cast(float, u & 0xffff0000u), 0x1p-126f, a),
+                     __builtin_amdgcn_fmed3f(b - __builtin_bit_cast(float, v & 0xffff0000u), 0x1p-126f, b)};
+    rest = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, bf16x2));
+  }
 }
 
 // The larger of the four 16-lane groups' values, on every lane: swapped halves
@@ -427,8 +431,8 @@ __device__ __forceinline__ float groups_max(float x) {
 }
 
 // What a weight of 1 goes to the matrix steps as, and counts as in its sum. f16
-// holds 2^-24 at least and 65504 at most: as 2^14 a weight loses at most 2^-39
-// there, and 2^20 of them 2^-19; as 1 they would lose 2^-5.
+// holds 2^-24 at least and 65504 at most: as 2^14 a small weight loses at most
+// 2^-39 there, and 2^20 of them 2^-19; as 1 they would lose 2^-5.
 template <typename T>
 constexpr float kLift = std::is_same_v<T, f16_t> ? 16384.f : 1.f;
 
@@ -577,18 +581,17 @@ __device__ __forceinline__ void use_tile(float scale2, Tile<T, D>& t, Heads<T, D
 #pragma unroll
     for (int r = 0; r < 4; ++r) x[h][r] = __builtin_amdgcn_exp2f(x[h][r] - ref) * kLift<T>;
   if constexpr (Sh::kHalf) {
-    // A weight goes to the matrix steps in two pieces of the type, what the
-    // first leaves in the second: to the square of the type's rounding. They are
-    // summed as they are, so that a key of all the weight answers its value.
-    // (64 sequences of 32 to 4064 keys, bf16: 107.7 us, a relative error of 1.7e-3
-    // that is the result's rounding; in one piece 107.4 us and 2.1e-3.)
+    // A weight goes to the matrix steps in two pieces. They are summed as they
+    // are, so that a key of all the weight answers its value. (64 sequences of 32
+    // to 4064 keys, bf16: 107.3 us, a relative error of 1.7e-3 that is the result's
+    // rounding; in one piece 107.4 us and 2.1e-3.)
     u32x4 p, rest;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float w0 = x[i / 2][2 * (i % 2)], w1 = x[i / 2][2 * (i % 2) + 1];
-      p[i] = pack2<T>(w0, w1);
-      const f32x2 held = unpack2<T>(p[i]);
-      rest[i] = pack2<T>(w0 - held[0], w1 - held[1]);
+      uint32_t first, second;
+      split2<T>(x[i / 2][2 * (i % 2)], x[i / 2][2 * (i % 2) + 1], first, second);
+      p[i] = first;
+      rest[i] = second;
     }
     constexpr uint32_t one = std::is_same_v<T, f16_t> ? 0x3c003c00u : 0x3f803f80u;
     st.l4 = mfma16<T>(u32x4{one, one, one, one}, p, st.l4);

@@ -283,6 +283,32 @@ def test_paged_attention_many_small_weights(client, dtype, group):
     close(got, want, (2 * ((n + 56) * W + u2) + U[dtype]) * want)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("dim,group,size", [(64, 2, 16), (128, 20, 16), (256, 1, 8), (96, 3, 24), (40, 2, 16)])
+def test_paged_attention_infinite_values(client, dtype, dim, group, size):
+    """An attended key's infinite value makes its column's answer infinite, two
+    of either sign, or a NaN, make it NaN; the other columns are as without."""
+    rng = np.random.default_rng(dim)
+    lengths = [50, 300, 33]
+    k, v, table = cache(rng, lengths, 1, size, dim, dtype, poison=False)
+    q = put(0.3 * rng.standard_normal((3, group, dim)), dtype)
+    plain = P.paged_attention(val(q), val(k), val(v), table, lengths)
+    vf = val(v)
+    vf[table[0, 1], 0, 1, 3] = np.inf
+    vf[table[1, 0], 0, 2, 5], vf[table[1, 2], 0, 1, 5] = np.inf, -np.inf
+    vf[table[1, 1], 0, 0, 7] = -np.inf
+    vf[table[2, 0], 0, 0, 9], vf[table[2, 0], 0, 1, 11] = np.nan, np.inf
+    n = np.array(lengths, np.int32)
+    (got,) = call(client, lambda b, p: b.paged_attention(*p), [q, k, put(vf, dtype), table, n], [dtype] * 3 + ["s32"] * 2)
+    got = val(got)
+    assert np.isposinf(got[0, :, 3]).all() and np.isneginf(got[1, :, 7]).all() and np.isposinf(got[2, :, 11]).all()
+    assert np.isnan(got[1, :, 5]).all() and np.isnan(got[2, :, 9]).all()
+    special = np.zeros((3, group, dim), bool)
+    special[0, :, 3] = special[1, :, [5, 7]] = special[2, :, [9, 11]] = True
+    tol = attention_tolerance(q, k, v, plain, dtype, dim ** -0.5, 300)
+    assert (np.abs(got - plain) <= tol)[~special].all()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("size,dim", [(8, 64), (16, 128), (48, 64), (5, 96), (7, 40)])
 def test_paged_attention_full_tables_at_the_pools_end(client, dtype, size, dim):
