@@ -205,7 +205,8 @@ __global__ void __launch_bounds__(kThreads, kTop ? 5 : 8)
       // y = d log2(e) + r by one fma, r what rounding m log2(e) left (a fma
       // gives it exactly). The chunk's sums give it back: over 2^r = 1 + c, |c|
       // below 2^-17, to c^2. The largest element's 1 + c becomes 1, so that no
-      // sum is below 1 and no log probability above 0.
+      // sum is below 1 and no log probability above 0; a sum of e^d d above 0 is
+      // rounding, and no entropy is below 0.
       const float ref2 = ref * kLog2e, r = fmaf(ref, kLog2e, -ref2);
       float l2 = 0.f, a2 = 0.f;
 #pragma unroll
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, kTop ? 5 : 8)
       const float c = __builtin_amdgcn_exp2f(r) - 1.f;
       a2 = fmaf(-r, l2, a2);
       s.l += fmaf(-c, l2, l2);
-      s.a = fmaf(fmaf(-c, a2, a2), kLn2, s.a);
+      s.a = fmaf(__builtin_elementwise_minimum(fmaf(-c, a2, a2), 0.f), kLn2, s.a);
     } else {
 #pragma unroll
       for (int i = 0; i < NV; ++i)

@@ -788,6 +788,16 @@ def test_token_logprobs_wherever_the_largest_logit_lies(client, dtype, vocab, k,
         assert np.array_equal(got[4][:, :equal], np.sort(at, 1))
 
 
+@pytest.mark.parametrize("vocab", [300, 9000, 40000])
+def test_token_logprobs_entropy_is_not_negative(client, vocab):
+    """0 where one token has all the weight, at a largest logit of any size."""
+    top = np.arange(-130, 130.5, 0.5)
+    x = np.repeat(top[:, None] - 110, vocab, 1).astype(np.float32)
+    x[:, 7] = top
+    got = call(client, lambda b, p: b.token_logprobs(*p), [x, np.full(len(top), 7, np.int32)], ["f32", "s32"])
+    assert (got[1] >= 0).all() and (got[1] <= W).all() and (got[0] == 0).all()
+
+
 # ---------------------------------------------------- the caller's addresses
 
 def _off(client, a, by):
